@@ -56,6 +56,11 @@ EXPORTS = {
     "eptq_rope_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, C.c_float, _vp]),
     "eptq_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "eptq_decode_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, C.c_float, _vp, _sz, _vp]),
+    "eptq_plan_pages": (_i, [_vp, _vp, _i, _vp, C.c_int64, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "eptq_rope_append_paged": (_i, [_i, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, _vp, C.c_int64, _vp, _vp, _vp,
+                                    _i, _i, _i, _i, _i, _i, C.c_float, _vp]),
+    "eptq_ragged_attention_workspace_bytes": (_sz, [_vp]),
+    "eptq_ragged_attention": (_i, [_vp, _vp, _sz, _vp]),
 }
 
 
@@ -82,6 +87,21 @@ class EptqFusion(C.Structure):
         ("x_op", C.c_int32), ("y_op", C.c_int32), ("norm_eps", C.c_float), ("rope_scaling", C.c_float),
         ("max_len", C.c_int32), ("reserved", C.c_int32),
         ("residual", _vp), ("position", _vp), ("inv_freq", _vp), ("x_aux", _vp),
+    ]
+
+
+EPTQ_FP16, EPTQ_BF16 = 0, 1
+
+
+class EptqAttention(C.Structure):
+    """struct EptqAttention of include/eptq_b200.h."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("batch", C.c_int32),
+        ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("max_rows", C.c_int32),
+        ("page_size", C.c_int32), ("n_pages", C.c_int32), ("table_width", C.c_int32),
+        ("scale", C.c_float), ("reserved", C.c_int32),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("table_stride", C.c_int64),
+        ("q", _vp), ("k", _vp), ("v", _vp), ("tables", _vp), ("kv_lens", _vp), ("cu_rows", _vp), ("out", _vp),
     ]
 
 

@@ -375,6 +375,77 @@ int eptq_decode_attention(const uint16_t* q, const uint16_t* k_cache,
                           size_t workspace_bytes, void* stream);
 
 /*
+ * Serving many requests from a paged key/value cache.  (No counterpart in the reference, which decodes
+ * through the HuggingFace cache.)  A cache is (n_pages, n_kv_heads, page_size, head_dim), one for keys and
+ * one for values; page_size a power of two from 16 to 128.  A request's page table names the pages that hold
+ * its tokens in order.  Lengths and tables live on the device: no call needs them on the host, so a step can
+ * be captured once and replayed for other lengths.  `dtype` is EPTQ_FP16 or EPTQ_BF16.
+ */
+enum { EPTQ_FP16 = 0, EPTQ_BF16 = 1 };
+
+/*
+ * Pages and slots for the new tokens of B requests, from their lengths.  Request b holds cached[b] tokens in
+ * the pages its row of `tables` (B rows of `width` page ids, table_stride apart) names, and gets fresh[b]
+ * more.  Pages are taken from the end of the first *n_free of `free_cap` page ids, in the order of the
+ * requests, and written into `tables`; what is left is *n_free_out (not n_free itself).
+ *   cu_rows   (B + 1): rows of request b are cu_rows[b] .. cu_rows[b+1]-1, at most `rows`.
+ *   kv_lens   (B): cached + fresh, or 0 where the request was not served.
+ *   positions, slots  (rows): the row's place in its request, and page * page_size + place in the page.
+ * A request is not served if its tokens need more than `width` pages, if its rows end behind `rows`, or if
+ * the free pages do not last up to it (a request that needs none is served all the same): it gets no page
+ * and its slots are -1.  Rows behind the last request have position 0 and slot -1.  Negative lengths count
+ * as 0.  All arrays on the device.
+ */
+int eptq_plan_pages(const int32_t* cached, const int32_t* fresh, int B, int32_t* tables, int64_t table_stride,
+                    int width, const int32_t* free_pages, int free_cap, const int32_t* n_free, int page_size,
+                    int rows, int32_t* cu_rows, int32_t* kv_lens, int64_t* positions, int64_t* slots,
+                    int32_t* n_free_out, void* stream);
+
+/*
+ * Rotary embedding of q and k, and the store of k and v into the pages.  Row r of q (rows, n_heads*head_dim)
+ * is rotated to q_out (contiguous; may be q where q is contiguous), row r of k goes rotated, row r of v as it
+ * is, to slot slots[r]; a slot outside the cache is not written.  Pairs (i, i + head_dim/2), angle
+ * positions[r] * inv_freq[i] formed and reduced in 64 bits, cos and sin times `scaling` kept in 32.
+ * Rows of q, k, v are q_stride, k_stride, v_stride elements apart (multiples of 8), pages page_stride elements
+ * (a multiple of 8).  head_dim a multiple of 16 up to 256.  Slots differ from one another.
+ */
+int eptq_rope_append_paged(int dtype, const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                           const uint16_t* v, int64_t v_stride, uint16_t* q_out, uint16_t* k_cache,
+                           uint16_t* v_cache, int64_t page_stride, const int64_t* positions, const int64_t* slots,
+                           const float* inv_freq, int rows, int n_heads, int n_kv_heads, int head_dim,
+                           int n_pages, int page_size, float scaling, void* stream);
+
+/*
+ * Causal attention of many requests' rows: request b owns the rows cu_rows[b] .. cu_rows[b+1]-1 of q and out.
+ *   page_size != 0: k and v are caches; the request has kv_lens[b] keys and its rows are the last of them, so
+ *     row t of n sees the keys 0 .. kv_lens[b] - n + t.  A row that sees none gives zeros.  Keys on a page id
+ *     outside the cache do not count.
+ *   page_size == 0: k and v (rows, n_kv_heads*head_dim) are packed like q, and row t sees the rows 0 .. t of
+ *     its request.
+ * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads); sums, maxima and
+ * products accumulate in 32 bits.  Rows behind the last request are left as they were.  head_dim 64 or 128.
+ * Scratch: eptq_ragged_attention_workspace_bytes, 256-byte aligned, its first 4 KB zero before the first use
+ * and left at zero; calls that may overlap on the GPU need scratch of their own.
+ */
+typedef struct EptqAttention {
+    int32_t dtype;                     /* of q, k, v and out                                             */
+    int32_t rows, batch;               /* rows of q and out; requests                                    */
+    int32_t n_heads, n_kv_heads, head_dim;
+    int32_t max_rows;                  /* most rows of one request: chooses the kernel, not the result   */
+    int32_t page_size, n_pages, table_width;          /* paged only                                     */
+    float scale;
+    int32_t reserved;
+    int64_t q_stride, k_stride, v_stride;             /* elements from row to row; paged: k, v page to page */
+    int64_t table_stride;
+    const uint16_t *q, *k, *v;
+    const int32_t *tables, *kv_lens, *cu_rows;
+    uint16_t* out;                     /* (rows, n_heads*head_dim), contiguous                           */
+} EptqAttention;
+
+size_t eptq_ragged_attention_workspace_bytes(const EptqAttention* a);
+int eptq_ragged_attention(const EptqAttention* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Un-quantized output projection fused with the greedy pick.  The reference keeps
  * lm_head in fp16 (quantize.py:86-90) and picks the token from the logits of a
  * library GEMM (bench_decode.py:35-41).  W fp16 (V, H) row-major, x fp16 (B, H);
