@@ -102,6 +102,7 @@ class EptqAttention(C.Structure):
         ("scale", C.c_float), ("reserved", C.c_int32),
         ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("table_stride", C.c_int64),
         ("q", _vp), ("k", _vp), ("v", _vp), ("tables", _vp), ("kv_lens", _vp), ("cu_rows", _vp), ("out", _vp),
+        ("status", _vp),
     ]
 
 

@@ -8,6 +8,10 @@
 #include "pair16.cuh"
 
 namespace eptq {
+
+size_t attention_tcgen05_bytes(const EptqAttention& a);
+int launch_attention_tcgen05(const EptqAttention& a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 namespace {
 
 constexpr int kSimpleWarps = 4;
@@ -28,7 +32,7 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) ragged_attention_simple_ker
     if (lo == a.batch) return;
     const int b = lo, first = a.cu_rows[b], n = a.cu_rows[b + 1] - first, t = r - first;
     const long long keys = a.page_size != 0 ? min(static_cast<long long>(a.kv_lens[b]), static_cast<long long>(a.table_width) * a.page_size) : n;
-    const long long seen = a.page_size != 0 ? min(a.kv_lens[b] - static_cast<long long>(n) + t + 1, keys) : t + 1;
+    const long long seen = keys - n + t + 1;
     const int g = h / (a.n_heads / a.n_kv_heads);
     float q[2 * W], o[2 * W], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -96,15 +100,23 @@ int check(const EptqAttention& a) {
 
 using namespace eptq;
 
+// Rows of one key/value head of a request from which the tensor-core kernel takes a paged call.
+constexpr int kTensorRows = 32;
+
+static bool on_tensor_cores(const EptqAttention& a) {
+    if (a.page_size == 0) return true;
+    return a.n_pages > 0 && static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > kTensorRows;
+}
+
 extern "C" size_t eptq_ragged_attention_workspace_bytes(const EptqAttention* a) {
-    return a == nullptr || check(*a) != EPTQ_OK ? 0 : kPartialOffset;
+    return a == nullptr || check(*a) != EPTQ_OK || !on_tensor_cores(*a) ? 0 : attention_tcgen05_bytes(*a);
 }
 
 extern "C" int eptq_ragged_attention(const EptqAttention* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (a == nullptr) return EPTQ_ERR_NULL;
     if (const int st = check(*a); st != EPTQ_OK) return st;
     if (a->rows == 0 || a->batch == 0) return EPTQ_OK;
-    (void)workspace; (void)workspace_bytes;
+    if (on_tensor_cores(*a)) return launch_attention_tcgen05(*a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
     const long long blocks = (static_cast<long long>(a->rows) * a->n_heads + kSimpleWarps - 1) / kSimpleWarps;
     if (blocks > 2147483647LL) return EPTQ_ERR_SHAPE;
     auto* kernel = a->dtype == EPTQ_FP16 ? (a->head_dim == 128 ? ragged_attention_simple_kernel<__half, 128> : ragged_attention_simple_kernel<__half, 64>)

@@ -25,6 +25,7 @@ from . import workspace_for
 
 __all__ = ["PagePlan", "plan_pages", "rope_append_paged", "paged_attention", "prompt_attention"]
 
+_STATUS_WORD = 4092          # byte of the scratch buffers' status word: the last counter
 _DTYPES = {torch.float16: _lib.EPTQ_FP16, torch.bfloat16: _lib.EPTQ_BF16}
 
 
@@ -167,9 +168,12 @@ def _attention(a: "_lib.EptqAttention", q: torch.Tensor, cu_rows: torch.Tensor, 
     a.scale = float(scale if scale is not None else a.head_dim ** -0.5)
     a.q_stride, a.q, a.cu_rows, a.out = _row_stride(q), q.data_ptr(), cu_rows.data_ptr(), out.data_ptr()
     with torch.cuda.device(q.device):
+        # Scratch of its own for every call, from torch's allocator: calls on different streams, and graphs captured on one
+        # stream and replayed on others, share none.  The status word is the framework's (see workspace_status_all).
+        a.status = workspace_for(q.device, 1 << 20).data_ptr() + _STATUS_WORD
         need = lib.eptq_ragged_attention_workspace_bytes(C.byref(a))
-        ws = workspace_for(q.device, need)
-        st = lib.eptq_ragged_attention(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q.device))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        st = lib.eptq_ragged_attention(C.byref(a), ws.data_ptr() if need else None, need, _stream(q.device))
     _lib.check(st, "eptq ragged attention")
     return out
 

@@ -424,8 +424,9 @@ int eptq_rope_append_paged(int dtype, const uint16_t* q, int64_t q_stride, const
  *     its request.
  * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads); sums, maxima and
  * products accumulate in 32 bits.  Rows behind the last request are left as they were.  head_dim 64 or 128.
- * Scratch: eptq_ragged_attention_workspace_bytes, 256-byte aligned, its first 4 KB zero before the first use
- * and left at zero; calls that may overlap on the GPU need scratch of their own.
+ * Keys of a paged request are at most table_width * page_size: a larger kv_lens[b] counts as that.
+ * Scratch: eptq_ragged_attention_workspace_bytes (0: none needed), 256-byte aligned, of any contents; calls that
+ * may overlap on the GPU need scratch of their own.
  */
 typedef struct EptqAttention {
     int32_t dtype;                     /* of q, k, v and out                                             */
@@ -440,6 +441,7 @@ typedef struct EptqAttention {
     const uint16_t *q, *k, *v;
     const int32_t *tables, *kv_lens, *cu_rows;
     uint16_t* out;                     /* (rows, n_heads*head_dim), contiguous                           */
+    int32_t* status;                   /* gets EPTQ_ERR_TIMEOUT if a bounded device-side wait runs out, or NULL */
 } EptqAttention;
 
 size_t eptq_ragged_attention_workspace_bytes(const EptqAttention* a);
