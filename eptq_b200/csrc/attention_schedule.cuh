@@ -2,7 +2,7 @@
 // the device knows.
 //
 // A request with n new rows behind `past` keys has, for every group of `hp` query heads that share their keys, row tiles
-// of `tile` tokens; a tile reads the keys its last row sees, in blocks of kKeyBlock.  All blocks of keys of all tiles form one
+// of `tile` tokens; a tile reads the keys its last row sees, in blocks of `kb`.  All blocks of keys of all tiles form one
 // sequence -- request, head group, row tile, block -- and launch block c takes the blocks from cut(c) to cut(c + 1).  Cuts
 // at equal distances balance requests of any lengths without knowing them on the host; a tile cut in two or more is joined
 // from partial results.  Joining costs about as much as a few blocks, so a cut moves to the end of a tile that is short or near.
@@ -17,8 +17,6 @@
 #endif
 
 namespace eptq {
-
-constexpr int kKeyBlock = 128;
 
 struct CutRule {
     int least;     // a tile of at most this many blocks is not cut
@@ -46,10 +44,10 @@ EPTQ_HD Request request_from(int row0, int row1, int rows, long long kv_len, lon
 EPTQ_HD int tiles_of(const Request& r, int tile) { return (r.n + tile - 1) / tile; }
 
 // Blocks of keys that row tile i reads (one at least: rows without keys are written too).
-EPTQ_HD int blocks_of(const Request& r, int tile, int i) {
+EPTQ_HD int blocks_of(const Request& r, int tile, int kb, int i) {
     const long long rows = static_cast<long long>(i + 1) * tile < r.n ? static_cast<long long>(i + 1) * tile : r.n;
     const long long keys = r.past + rows;
-    return keys <= kKeyBlock ? 1 : static_cast<int>((keys + kKeyBlock - 1) / kKeyBlock);
+    return keys <= kb ? 1 : static_cast<int>((keys + kb - 1) / kb);
 }
 
 // sum of floor((a i + b) / m) for i = 0 .. n-1, a, b >= 0: the usual exchange of the axes under the line
@@ -70,16 +68,16 @@ EPTQ_HD long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
 }
 
 // Blocks of the row tiles before tile i, i <= tiles_of.
-EPTQ_HD long long blocks_before(const Request& r, int tile, int i) {
+EPTQ_HD long long blocks_before(const Request& r, int tile, int kb, int i) {
     if (i <= 0) return 0;
     const int full = static_cast<long long>(i) * tile <= r.n ? i : i - 1;        // tiles that are not cut off by the request's end
     int z = r.past < 0 ? -r.past / tile : 0;                                      // tiles without keys: one block each
     if (z > full) z = full;
     long long sum = z;
     if (full > z)
-        sum += floor_sum(static_cast<unsigned>(full - z), kKeyBlock, static_cast<unsigned>(tile),
-                         static_cast<unsigned>(r.past + static_cast<long long>(z + 1) * tile + kKeyBlock - 1));
-    if (i > full) sum += blocks_of(r, tile, i - 1);
+        sum += floor_sum(static_cast<unsigned>(full - z), kb, static_cast<unsigned>(tile),
+                         static_cast<unsigned>(r.past + static_cast<long long>(z + 1) * tile + kb - 1));
+    if (i > full) sum += blocks_of(r, tile, kb, i - 1);
     return sum;
 }
 
@@ -90,20 +88,20 @@ struct Place {
 };
 
 // x = blocks of the request before the place, 0 <= x < groups * blocks_before(all tiles).
-EPTQ_HD Place place_of(const Request& r, int tile, long long x) {
+EPTQ_HD Place place_of(const Request& r, int tile, int kb, long long x) {
     const int tiles = tiles_of(r, tile);
-    const long long per_group = blocks_before(r, tile, tiles);
+    const long long per_group = blocks_before(r, tile, kb, tiles);
     Place p;
     p.group = static_cast<int>(x / per_group);
     const long long y = x - p.group * per_group;
     int lo = 0, hi = tiles - 1;                       // the last tile that begins at or before y
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (blocks_before(r, tile, mid) <= y) lo = mid; else hi = mid - 1;
+        if (blocks_before(r, tile, kb, mid) <= y) lo = mid; else hi = mid - 1;
     }
     p.tile = lo;
-    p.block = static_cast<int>(y - blocks_before(r, tile, lo));
-    p.blocks = blocks_of(r, tile, lo);
+    p.block = static_cast<int>(y - blocks_before(r, tile, kb, lo));
+    p.blocks = blocks_of(r, tile, kb, lo);
     return p;
 }
 

@@ -23,24 +23,20 @@
 //
 // TMEM: S/P of half 0 at column 0, of half 1 at 128; O of half 0 at 256, of half 1 at 256 + head_dim.
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <mutex>
 
 #include "attention_args.cuh"
+#include "attention_host.cuh"
 #include "pair16.cuh"
 
 namespace eptq {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kKeyBlock = 128;
 constexpr int kItems = 4;                      // ring of items
 constexpr int kMaxSlots = 10;
 constexpr int kKeysSeen = 16;                  // ring of per-block page flags
-constexpr unsigned long long kWaitNs = 2000000000ull;
-constexpr float kExpOffset = 7.f;
-constexpr float kRescaleAt = 8.f;
 
 // Q: two halves of 128 rows; K and V: slots of 128 keys; each in head_dim / 64 boxes of 128-byte rows.
 __host__ __device__ constexpr int tile_bytes(int hd) { return 128 * hd * 2; }
@@ -48,50 +44,6 @@ __host__ __device__ constexpr int slots(int hd) { return hd == 128 ? 5 : 10; }
 __host__ __device__ constexpr int smem_bytes(int hd) { return (2 + slots(hd)) * tile_bytes(hd) + 1024; }
 static_assert(slots(64) <= kMaxSlots && slots(128) <= kMaxSlots, "barrier array");
 
-struct Item {
-    int row, tokens, head, request;    // first row, tokens that exist, first query head; request < 0: no more items
-    int seen;                          // last key that the first token sees
-    int keys;                          // keys of the request that the tile's last token sees
-    int block, blocks;                 // first block of keys, number of blocks
-    int count[2];                      // blocks of either half
-    int slot;                          // where its partial result goes, -1: it is the whole tile
-    int pad;
-};
-
-__device__ __forceinline__ unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(unsigned bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_expect_tx(unsigned bar, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
-}
-// Bounded by the global timer; a wait that runs out raises `stop`, which ends the other warps' waits as well.
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int* stop) {
-    unsigned long long t0 = 0;
-    for (unsigned it = 0;; ++it) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
-        if ((it & 255u) == 255u) {
-            if (*stop) return false;
-            unsigned long long now;
-            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitNs) { *stop = 1; return false; }
-        }
-    }
-}
-// The same for a whole warp: all lanes agree on the outcome.
-__device__ __forceinline__ bool warp_wait(unsigned bar, unsigned parity, volatile int* stop) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop));
-}
 __device__ __forceinline__ void commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
@@ -148,31 +100,17 @@ __device__ __forceinline__ void tmem_st32(unsigned addr, const unsigned* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void tma_3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tma_4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
-}
-
-__device__ __forceinline__ Request load_request(const AttentionArgs& p, int b, bool paged) {
-    return request_from(__ldg(p.cu_rows + b), __ldg(p.cu_rows + b + 1), p.rows, paged ? __ldg(p.kv_lens + b) : 0, p.table_keys, paged);
-}
+// An item and the blocks of keys that either half of its rows sees.
+struct HalvedItem {
+    Item it;
+    int count[2];
+};
 
 struct Shared {
     unsigned long long q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
     unsigned long long kv_full[kMaxSlots], kv_empty[kMaxSlots], item_full[kItems], item_empty[kItems];
-    Item items[kItems];
-    long long scan[kThreads / 32 + 1];
-    long long place_before[2];             // blocks before the request that holds the share's begin and end
-    int place_request[2];
+    HalvedItem items[kItems];
+    ShareScratch<kThreads> share;
     unsigned lost[kKeysSeen];              // 16-key groups of a block that are on no page of the cache
     unsigned tmem;
     int stop;
@@ -189,8 +127,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
     unsigned char* const tiles = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int share_id = blockIdx.x, n_shares = gridDim.x;
-    const int tile_tokens = 2 * p.tokens_per_half, groups = p.n_heads / p.heads_per_tile;
+    const int tile_tokens = 2 * p.tokens_per_half;
 
     if (tid == 0) {
         for (int h = 0; h < 2; ++h) {
@@ -218,62 +155,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---------------- this block's share: blocks of all requests summed, then the requests that hold its two ends
-    long long all = 0, share = 0, mine[2] = {0, 0};
-    for (int pass = 0; pass < 2; ++pass) {
-        long long before = 0;
-        for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-            const int b = b0 + tid;
-            long long w = 0;
-            if (b < p.batch) {
-                const Request r = load_request(p, b, PAGED);
-                w = blocks_before(r, tile_tokens, tiles_of(r, tile_tokens)) * groups;
-            }
-            long long ends = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long up = __shfl_up_sync(0xffffffffu, ends, o);
-                if (lane >= o) ends += up;
-            }
-            __syncthreads();
-            if (lane == 31) sh.scan[warp] = ends;
-            __syncthreads();
-            long long chunk = 0;
-#pragma unroll
-            for (int i = 0; i < kThreads / 32; ++i) {
-                if (i == warp) ends += chunk;
-                chunk += sh.scan[i];
-            }
-            ends += before;
-            if (pass == 0 && b0 + kThreads >= p.batch) {          // the sum is known: this chunk may hold the ends already
-                all = before + chunk;
-                share = share_of(all, n_shares, rule);
-                mine[0] = share_id * share;
-                mine[1] = share_id + 1 < n_shares ? mine[0] + share : all;
-            }
-            if (pass == 1 || b0 + kThreads >= p.batch)
-                for (int e = 0; e < 2; ++e)
-                    if (mine[e] < ends && mine[e] >= ends - w) { sh.place_request[e] = b; sh.place_before[e] = ends - w; }
-            before += chunk;
-        }
-        if (p.batch <= kThreads) break;                           // one chunk: both passes in one
-    }
-    __syncthreads();
-    long long cut[2];
-    Place at[2];
-    int request0 = 0;
-    for (int e = 0; e < 2; ++e) {                                  // every thread alike: the values are needed by all
-        cut[e] = all;
-        if (mine[e] < all) {
-            const int b = sh.place_request[e];
-            const Request r = load_request(p, b, PAGED);
-            at[e] = place_of(r, tile_tokens, mine[e] - sh.place_before[e]);
-            cut[e] = mine[e] + moved(at[e], rule);
-            if (e == 0) request0 = b;
-        }
-    }
-    if (cut[0] >= cut[1]) {                                        // nothing left for this block
-        if (tid == 0 && p.cut_tiles != nullptr) p.cut_tiles[share_id].of = 0;
+    const Share share = find_share<kThreads, 1>(p, tile_tokens, kKeyBlock, rule, sh.share);
+    if (share.begin >= share.end) {                                // nothing left for this block
+        if (tid == 0 && p.cut_tiles != nullptr) p.cut_tiles[blockIdx.x].of = 0;
         return;
     }
 
@@ -291,66 +175,40 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             // ---------------- items and loads
-            int b = request0;
-            Request r = load_request(p, b, PAGED);
-            Place now = at[0];
-            int step = moved(at[0], rule);
-            if (step == now.blocks - now.block && step != 0) { now.block = 0; ++now.tile; } else now.block += step;
-            long long left = cut[1] - cut[0], flat = cut[0];
+            ShareWalk walk;
+            walk.start(p, share);
             unsigned kv_seq = 0, n_items = 0, q_count[2] = {0, 0}, block_seq = 0;
             bool cut_written = false;
             for (;;) {
-                // the next tile that exists
-                int row_tiles = tiles_of(r, tile_tokens);
-                if (now.tile >= row_tiles) { now.tile = 0; ++now.group; }
-                while (left > 0 && (row_tiles == 0 || now.group >= groups)) {
-                    r = load_request(p, ++b, PAGED);
-                    row_tiles = tiles_of(r, tile_tokens);
-                    now.group = now.tile = 0;
-                }
+                HalvedItem hit;
+                Item& it = hit.it;
+                const bool more = walk.next(p, tile_tokens, kKeyBlock, rule, it);
                 const int ring = n_items % kItems;
                 ok = warp_wait(smem_u32(&sh.item_empty[ring]), ((n_items / kItems) & 1u) ^ 1u, &sh.stop);
                 if (!ok) break;
-                if (left <= 0) {
+                if (!more) {
                     if (lane == 0) {
-                        sh.items[ring].request = -1;
+                        sh.items[ring].it.request = -1;
                         mbar_arrive(smem_u32(&sh.item_full[ring]));
                     }
                     break;
                 }
-                const int blocks = blocks_of(r, tile_tokens, now.tile);
-                Item it;
-                it.request = b;
-                it.row = r.first + now.tile * tile_tokens;
-                it.tokens = min(tile_tokens, r.n - now.tile * tile_tokens);
-                it.head = now.group * p.heads_per_tile;
-                it.seen = r.past + now.tile * tile_tokens;
-                it.keys = max(0, it.seen + it.tokens);
-                it.block = now.block;
-                it.blocks = static_cast<int>(min(static_cast<long long>(blocks - now.block), left));
                 // half 0 sees fewer keys than half 1; a half without tokens has no blocks
                 const int keys0 = it.seen + min(it.tokens, p.tokens_per_half);
                 const int need0 = keys0 <= kKeyBlock ? 1 : (keys0 + kKeyBlock - 1) / kKeyBlock;
-                it.count[0] = max(0, min(it.blocks, need0 - it.block));
-                it.count[1] = it.tokens > p.tokens_per_half ? it.blocks : 0;
-                const bool whole = it.blocks == blocks;
-                it.slot = whole ? -1 : 2 * share_id + (it.block == 0 ? 1 : 0);
-                it.pad = 0;
+                hit.count[0] = max(0, min(it.blocks, need0 - it.block));
+                hit.count[1] = it.tokens > p.tokens_per_half ? it.blocks : 0;
                 if (lane == 0) {
-                    sh.items[ring] = it;
+                    sh.items[ring] = hit;
                     mbar_arrive(smem_u32(&sh.item_full[ring]));
-                    if (!whole && it.block == 0) {
-                        CutTile c;
-                        c.of = last_share(flat + blocks, share, rule) - share_id + 1;
-                        c.row = it.row; c.tokens = it.tokens; c.head = it.head;
-                        c.pad[0] = c.pad[1] = c.pad[2] = c.pad[3] = 0;
-                        p.cut_tiles[share_id] = c;
+                    if (it.of > 0) {
+                        write_cut_tile(p, it);
                         cut_written = true;
                     }
                 }
                 ++n_items;
                 for (int h = 0; h < 2 && ok; ++h) {
-                    if (it.count[h] == 0) continue;
+                    if (hit.count[h] == 0) continue;
                     ok = warp_wait(smem_u32(&sh.q_empty[h]), (q_count[h] & 1u) ^ 1u, &sh.stop);
                     if (!ok) break;
                     ++q_count[h];
@@ -362,7 +220,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                 }
                 const int kv_head = it.head / p.kv_group;
-                const int last_key = it.keys;
                 int table_at = -1, page_id = 0;                    // table columns table_at .. table_at + 31, one per lane
                 for (int j = 0; j < it.blocks && ok; ++j) {
                     const int key0 = (it.block + j) * kKeyBlock;
@@ -370,11 +227,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     unsigned lost = 0;
                     if (PAGED) {
                         // this block's pages: lane i holds page i
-                        pages = (max(0, min(kKeyBlock, last_key - key0)) + p.page_size - 1) / p.page_size;
+                        pages = (max(0, min(kKeyBlock, it.keys - key0)) + p.page_size - 1) / p.page_size;
                         const int col = key0 / p.page_size;
                         if (table_at < 0 || col < table_at || col + pages > table_at + 32) {
                             table_at = col;
-                            page_id = col + lane < p.table_width ? __ldg(p.tables + b * p.table_stride + col + lane) : -1;
+                            page_id = col + lane < p.table_width ? __ldg(p.tables + it.request * p.table_stride + col + lane) : -1;
                         }
                         page = __shfl_sync(0xffffffffu, page_id, (col - table_at + lane) & 31);
                         const bool gone = lane < pages && (page < 0 || page >= p.n_pages);
@@ -404,17 +261,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         } else if (lane == 0) {
                             mbar_arrive_expect_tx(bar, kTile);
                             for (int x = 0; x < kBoxes; ++x)
-                                tma_3d(dst + x * kBox, map, x * 64, kv_head, r.first + key0, bar);
+                                tma_3d(dst + x * kBox, map, x * 64, kv_head, walk.r.first + key0, bar);
                         }
                     }
                 }
                 if (!ok) break;
-                left -= it.blocks;
-                flat += it.blocks;
-                now.block = 0;
-                ++now.tile;
             }
-            if (lane == 0 && !cut_written && p.cut_tiles != nullptr) p.cut_tiles[share_id].of = 0;
+            if (lane == 0 && !cut_written && p.cut_tiles != nullptr) p.cut_tiles[blockIdx.x].of = 0;
             if (!ok) {
                 // copies still in flight write shared memory: wait for them before it is given up
                 __syncwarp();
@@ -433,9 +286,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int ring = n_items % kItems;
                 ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
                 if (!ok) break;
-                const int request = sh.items[ring].request, blocks = sh.items[ring].blocks;
-                const int count[2] = {sh.items[ring].count[0], sh.items[ring].count[1]};
-                const int keys = sh.items[ring].keys - sh.items[ring].block * kKeyBlock;
+                const HalvedItem& hit = sh.items[ring];
+                const int request = hit.it.request, blocks = hit.it.blocks;
+                const int count[2] = {hit.count[0], hit.count[1]};
+                const int keys = hit.it.keys - hit.it.block * kKeyBlock;
                 if (request < 0) break;
                 ++n_items;
                 for (int j = 0; j <= blocks && ok; ++j) {
@@ -529,10 +383,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int ring = n_items % kItems;
             ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
             if (!ok) break;
-            const Item it = sh.items[ring];
+            const Item it = sh.items[ring].it;
+            const int count = sh.items[ring].count[h];
             if (it.request < 0) break;
             ++n_items;
-            const int count = it.count[h];
             const bool live_row = in_tile && token < it.tokens;
             const int seen = it.seen + min(token, it.tokens - 1);              // the last key this row sees
             float top = -INFINITY, bias = 0.f, sum = 0.f;                       // maximum of s; exponent = s * scale - bias
@@ -629,7 +483,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                 }
             } else if (it.tokens > h * p.tokens_per_half) {
-                float* const piece = p.partial + static_cast<long long>(it.slot) * (256 * (HD + 2));
+                float* const piece = p.partial + it.slot * piece_floats(256, HD);
                 const int at_row = h * 128 + row;
                 piece[256 * HD + at_row] = count > 0 ? bias : 0.f;
                 piece[256 * HD + 256 + at_row] = count > 0 ? sum : 0.f;
@@ -642,7 +496,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (!live_row) continue;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            reinterpret_cast<float4*>(piece)[(c * 8 + i) * 256 + at_row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            reinterpret_cast<float4*>(piece + at_row * HD)[c * 8 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
@@ -663,182 +517,55 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
-// ---- joining the pieces of cut tiles -------------------------------------------------------------------
-// Block (share, 32 rows of its cut tile), one warp per quarter of the head.  Pieces are added in the order of the keys.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionArgs p) {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const CutTile c = p.cut_tiles[blockIdx.x];
-    if (c.of == 0) return;
-    const int at_row = blockIdx.y * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
-    const int h = at_row >> 7, row = at_row & 127;
-    const int token = h * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
-    if (row >= p.heads_per_tile * p.tokens_per_half || token >= c.tokens) return;
-    constexpr int kVec = HD / 16;                                     // float4 of a quarter
-    constexpr long long kPiece = 256 * (HD + 2);
-    float top = -INFINITY;
-    for (int i = 0; i < c.of; ++i) {
-        const float* piece = p.partial + (2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kPiece + 256 * HD + at_row;
-        if (__ldcg(piece + 256) > 0.f) top = fmaxf(top, __ldcg(piece));
-    }
-    float4 o[kVec];
-    float sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < c.of; ++i) {
-        const float* piece = p.partial + (2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kPiece;
-        const float s = __ldcg(piece + 256 * HD + 256 + at_row);
-        if (s == 0.f) continue;                                       // no key seen: its o was not written
-        const float w = exp2_approx(__ldcg(piece + 256 * HD + at_row) - top);
-        sum += s * w;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(piece) + (part * kVec + v) * 256 + at_row);
-            o[v].x += x.x * w; o[v].y += x.y * w; o[v].z += x.z * w; o[v].w += x.w * w;
-        }
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    uint16_t* const dst = p.out + (static_cast<long long>(c.row + token) * p.n_heads + c.head + head) * HD + part * (HD / 4);
-#pragma unroll
-    for (int v = 0; v < kVec; v += 2) {
-        uint4 w;
-        w.x = Pair16<T>::pack(o[v].x * inv, o[v].y * inv);
-        w.y = Pair16<T>::pack(o[v].z * inv, o[v].w * inv);
-        w.z = Pair16<T>::pack(o[v + 1].x * inv, o[v + 1].y * inv);
-        w.w = Pair16<T>::pack(o[v + 1].z * inv, o[v + 1].w * inv);
-        *reinterpret_cast<uint4*>(dst + v * 4) = w;
-    }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, []() {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-            qres == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-    });
-    return fn;
-}
-
-// Boxes of 64 columns in 128-byte swizzle; what lies outside reads as zeros.  strides[i] in elements, of dims[i + 1].
-bool encode(CUtensorMap* map, const EptqAttention& a, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides, const cuuint32_t* box) {
-    cuuint64_t bytes[4];
-    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-    for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
-    return map_encoder()(map, a.dtype == EPTQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
-                         const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 constexpr CutRule kRule = {8, 2, 4};
-constexpr size_t kCutTileBytes = (kSms * sizeof(CutTile) + 255) / 256 * 256;
-
-size_t piece_bytes(int hd) { return static_cast<size_t>(256) * (hd + 2) * sizeof(float); }
-
-// Whether any tile may have more blocks than stay uncut, by what the host knows.
-bool may_cut(const EptqAttention& a) {
-    const long long keys = a.page_size != 0 ? static_cast<long long>(a.table_width) * a.page_size : a.rows;
-    return keys > static_cast<long long>(kRule.least) * kKeyBlock;
-}
-
-template <typename Args0, typename... Args>
-int launch(void (*kernel)(Args0, Args...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args0& a0, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, a0, args...) != cudaSuccess) {
-        cudaGetLastError();
-        return EPTQ_ERR_LAUNCH;
-    }
-    return EPTQ_OK;
-}
-
 template <typename T, int HD, bool PAGED>
-int run(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, bool join, int dev, cudaStream_t stream) {
+int run(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {
     static std::once_flag once[64];
     static bool set[64] = {};
     std::call_once(once[dev], [dev]() {
         set[dev] = cudaFuncSetAttribute(attention_tcgen05_kernel<T, HD, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(HD)) == cudaSuccess;
     });
     if (!set[dev]) return EPTQ_ERR_LAUNCH;
-    int st = launch(attention_tcgen05_kernel<T, HD, PAGED>, dim3(kSms), kThreads, smem_bytes(HD), stream, q, k, v, args, kRule);
-    if (st != EPTQ_OK) return st;
-    count_launch(EPTQ_KERNEL_OTHER);
-    if (!join) return EPTQ_OK;
-    st = launch(attention_join_kernel<T, HD>, dim3(kSms, 8), 128, 0, stream, args);
-    if (st == EPTQ_OK) count_launch(EPTQ_KERNEL_OTHER);
-    return st;
+    return launch_dependent(attention_tcgen05_kernel<T, HD, PAGED>, dim3(kSms), kThreads, smem_bytes(HD), stream, q, k, v, args, kRule);
 }
 
 }  // namespace
 
-size_t attention_tcgen05_bytes(const EptqAttention& a) {
-    return may_cut(a) ? kCutTileBytes + 2 * kSms * piece_bytes(a.head_dim) : 0;
+AttentionPlan attention_tcgen05_plan(const EptqAttention& a) {
+    AttentionPlan plan;
+    plan.shares = kSms;
+    plan.tile_rows = 256;
+    const long long keys = a.page_size != 0 ? static_cast<long long>(a.table_width) * a.page_size : a.rows;
+    plan.may_cut = keys > static_cast<long long>(kRule.least) * kKeyBlock;
+    return plan;
 }
 
-// Needs keys to exist as memory: a paged call with at least one page.
-int launch_attention_tcgen05(const EptqAttention& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-    if (map_encoder() == nullptr) return EPTQ_ERR_LAUNCH;
-    const bool paged = a.page_size != 0, join = may_cut(a);
-    if (join && (workspace == nullptr || workspace_bytes < attention_tcgen05_bytes(a))) return EPTQ_ERR_WORKSPACE;
-    if (join && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return EPTQ_ERR_ALIGN;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return EPTQ_ERR_LAUNCH;
-    AttentionArgs p = {};
-    p.tables = a.tables; p.kv_lens = a.kv_lens; p.cu_rows = a.cu_rows;
-    p.out = a.out; p.status = a.status;
-    p.cut_tiles = join ? static_cast<CutTile*>(workspace) : nullptr;
-    p.partial = join ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCutTileBytes) : nullptr;
-    p.table_stride = a.table_stride;
-    p.table_keys = static_cast<long long>(a.table_width) * a.page_size;
-    p.rows = a.rows; p.batch = a.batch; p.n_heads = a.n_heads;
-    p.kv_group = a.n_heads / a.n_kv_heads;
-    p.heads_per_tile = p.kv_group;                       // all heads of a key/value head, or as many of them as fit 128 rows
-    while (p.heads_per_tile > 128 || p.kv_group % p.heads_per_tile != 0) --p.heads_per_tile;
+int launch_attention_tcgen05(const EptqAttention& a, AttentionArgs& p, int dev, cudaStream_t stream) {
+    const bool paged = a.page_size != 0;
+    p.heads_per_tile = heads_in(p.kv_group, 128);
     p.tokens_per_half = 128 / p.heads_per_tile;
-    p.page_size = a.page_size; p.n_pages = a.n_pages; p.table_width = a.table_width;
-    // A scale of zero stays the smallest step above it: masked scores are -infinity and must stay so.
-    p.scale_log2 = a.scale == 0.f ? 1e-30f : (a.scale < 0.f ? -a.scale : a.scale) * kLog2e;
-    p.negative = a.scale < 0.f;
     CUtensorMap q, k, v;
     const cuuint64_t hd = a.head_dim, nkv = a.n_kv_heads;
     {
         const cuuint64_t dims[3] = {hd, static_cast<cuuint64_t>(a.n_heads), static_cast<cuuint64_t>(a.rows)};
         const int64_t strides[2] = {a.head_dim, a.q_stride};
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.heads_per_tile), static_cast<cuuint32_t>(p.tokens_per_half)};
-        if (!encode(&q, a, a.q, 3, dims, strides, box)) return EPTQ_ERR_LAUNCH;
+        if (!encode_map(&q, a.dtype, a.q, 3, dims, strides, box)) return EPTQ_ERR_LAUNCH;
     }
-    bool ok;
     if (paged) {
-        const cuuint64_t dims[4] = {hd, static_cast<cuuint64_t>(a.page_size), nkv, static_cast<cuuint64_t>(a.n_pages)};
-        const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.page_size), 1, 1};
-        const int64_t ks[3] = {a.head_dim, static_cast<int64_t>(a.page_size) * a.head_dim, a.k_stride};
-        const int64_t vs[3] = {a.head_dim, static_cast<int64_t>(a.page_size) * a.head_dim, a.v_stride};
-        ok = encode(&k, a, a.k, 4, dims, ks, box) && encode(&v, a, a.v, 4, dims, vs, box);
+        if (!encode_page_maps(&k, &v, a, a.page_size)) return EPTQ_ERR_LAUNCH;
     } else {
         const cuuint64_t dims[3] = {hd, nkv, static_cast<cuuint64_t>(a.rows)};
         const cuuint32_t box[3] = {64, 1, kKeyBlock};
         const int64_t ks[2] = {a.head_dim, a.k_stride}, vs[2] = {a.head_dim, a.v_stride};
-        ok = encode(&k, a, a.k, 3, dims, ks, box) && encode(&v, a, a.v, 3, dims, vs, box);
+        if (!encode_map(&k, a.dtype, a.k, 3, dims, ks, box) || !encode_map(&v, a.dtype, a.v, 3, dims, vs, box)) return EPTQ_ERR_LAUNCH;
     }
-    if (!ok) return EPTQ_ERR_LAUNCH;
     if (a.dtype == EPTQ_FP16) {
-        if (a.head_dim == 128) return paged ? run<__half, 128, true>(q, k, v, p, join, dev, stream) : run<__half, 128, false>(q, k, v, p, join, dev, stream);
-        return paged ? run<__half, 64, true>(q, k, v, p, join, dev, stream) : run<__half, 64, false>(q, k, v, p, join, dev, stream);
+        if (a.head_dim == 128) return paged ? run<__half, 128, true>(q, k, v, p, dev, stream) : run<__half, 128, false>(q, k, v, p, dev, stream);
+        return paged ? run<__half, 64, true>(q, k, v, p, dev, stream) : run<__half, 64, false>(q, k, v, p, dev, stream);
     }
-    if (a.head_dim == 128) return paged ? run<__nv_bfloat16, 128, true>(q, k, v, p, join, dev, stream) : run<__nv_bfloat16, 128, false>(q, k, v, p, join, dev, stream);
-    return paged ? run<__nv_bfloat16, 64, true>(q, k, v, p, join, dev, stream) : run<__nv_bfloat16, 64, false>(q, k, v, p, join, dev, stream);
+    if (a.head_dim == 128) return paged ? run<__nv_bfloat16, 128, true>(q, k, v, p, dev, stream) : run<__nv_bfloat16, 128, false>(q, k, v, p, dev, stream);
+    return paged ? run<__nv_bfloat16, 64, true>(q, k, v, p, dev, stream) : run<__nv_bfloat16, 64, false>(q, k, v, p, dev, stream);
 }
 
 }  // namespace eptq

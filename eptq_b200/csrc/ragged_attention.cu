@@ -1,81 +1,86 @@
-// Causal attention of many requests' rows, over a paged key/value cache or over packed keys and values.
+// Causal attention of many requests' rows, over a paged key/value cache or over packed keys and values: the entry point,
+// the choice of the kernel, and the join of row tiles whose keys several blocks have taken.
 //
 // For row t of a request with n rows and L keys, and head h with the keys of head g = h / (n_heads / n_kv_heads):
-//     o_t = sum_j exp(s_tj - m_t) v_j / sum_j exp(s_tj - m_t),   s_tj = scale q_t . k_j,   j = 0 .. L - n + t,
-// with the maximum m_t and the sum kept while the keys go by once.
+//     o_t = sum_j exp(s_tj - m_t) v_j / sum_j exp(s_tj - m_t),   s_tj = scale q_t . k_j,   j = 0 .. L - n + t.
+// A piece of the keys gives (reference m, sum, o); pieces join as sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) sum_i.
 
-#include "common.cuh"
+#include <mutex>
+
+#include "attention_host.cuh"
 #include "pair16.cuh"
 
 namespace eptq {
 
-size_t attention_tcgen05_bytes(const EptqAttention& a);
-int launch_attention_tcgen05(const EptqAttention& a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+PFN_cuTensorMapEncodeTiled_v12000 attention_map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, []() {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+            qres == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
 
 namespace {
 
-constexpr int kSimpleWarps = 4;
+// Block (share, 16 rows of its cut tile), 8 columns of one row per thread.  Pieces are added in the order of the keys.
+constexpr int kJoinRows = 16;
 
-// One warp per row and head, one key after the other.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kSimpleWarps * 32) ragged_attention_simple_kernel(const EptqAttention a) {
-    constexpr int W = HD / 64;                               // 32-bit words of a head that a lane holds
-    const int lane = threadIdx.x & 31;
-    const long long unit = blockIdx.x * static_cast<long long>(kSimpleWarps) + (threadIdx.x >> 5);
-    const int r = static_cast<int>(unit / a.n_heads), h = static_cast<int>(unit % a.n_heads);
-    if (r >= a.rows) return;
-    int lo = 0, hi = a.batch;                                // the request whose rows hold r
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu_rows[mid + 1] > r) hi = mid; else lo = mid + 1;
+__global__ void __launch_bounds__(kJoinRows * HD / 8) attention_join_kernel(const __grid_constant__ AttentionArgs p) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const CutTile c = p.cut_tiles[blockIdx.x];
+    if (c.of == 0) return;
+    const int at_row = blockIdx.y * kJoinRows + threadIdx.x / (HD / 8), col = threadIdx.x % (HD / 8) * 8;
+    const int half = at_row >> 7, row = at_row & 127;
+    const int token = half * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
+    if (row >= p.heads_per_tile * p.tokens_per_half || token >= c.tokens) return;
+    const long long size = piece_floats(p.tile_rows, HD);
+    const float* const first = p.partial + (2 * blockIdx.x + 1) * size;
+    const float* const others = p.partial + 2 * blockIdx.x * size;      // piece i at 2 i pieces behind, i = 1 ..
+    const int stat = p.tile_rows * HD + at_row;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int i = 0; i < c.of; ++i) {
+        const float* const piece = i == 0 ? first : others + 2 * i * size;
+        const float bias = __ldcg(piece + stat), sum = __ldcg(piece + stat + p.tile_rows);
+        if (sum != 0.f) top = fmaxf(top, bias);
     }
-    if (lo == a.batch) return;
-    const int b = lo, first = a.cu_rows[b], n = a.cu_rows[b + 1] - first, t = r - first;
-    const long long keys = a.page_size != 0 ? min(static_cast<long long>(a.kv_lens[b]), static_cast<long long>(a.table_width) * a.page_size) : n;
-    const long long seen = keys - n + t + 1;
-    const int g = h / (a.n_heads / a.n_kv_heads);
-    float q[2 * W], o[2 * W], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const float2 f = Pair16<T>::unpack(reinterpret_cast<const unsigned*>(a.q + r * a.q_stride + h * HD)[w * 32 + lane]);
-        q[2 * w] = f.x * a.scale; q[2 * w + 1] = f.y * a.scale;
-        o[2 * w] = o[2 * w + 1] = 0.f;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, all = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < c.of; ++i) {
+        const float* const piece = i == 0 ? first : others + 2 * i * size;
+        const float sum = __ldcg(piece + stat + p.tile_rows);
+        const float w = exp2_approx(__ldcg(piece + stat) - top);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(piece + at_row * HD + col));
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(piece + at_row * HD + col) + 1);
+        if (sum == 0.f) continue;                                       // no key seen: its o was not written
+        all += sum * w;
+        o[0] += x.x * w; o[1] += x.y * w; o[2] += x.z * w; o[3] += x.w * w;
+        o[4] += y.x * w; o[5] += y.y * w; o[6] += y.z * w; o[7] += y.w * w;
     }
-    for (long long j = 0; j < seen; ++j) {
-        long long k_at, v_at;
-        if (a.page_size != 0) {
-            const int page = a.tables[b * a.table_stride + j / a.page_size];
-            if (page < 0 || page >= a.n_pages) continue;
-            const long long in_page = (static_cast<long long>(g) * a.page_size + j % a.page_size) * HD;
-            k_at = page * a.k_stride + in_page;
-            v_at = page * a.v_stride + in_page;
-        } else {
-            k_at = (first + j) * a.k_stride + g * HD;
-            v_at = (first + j) * a.v_stride + g * HD;
-        }
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 f = Pair16<T>::unpack(reinterpret_cast<const unsigned*>(a.k + k_at)[w * 32 + lane]);
-            s = fmaf(q[2 * w], f.x, fmaf(q[2 * w + 1], f.y, s));
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float m2 = fmaxf(m, s);
-        const float keep = m2 == -INFINITY ? 1.f : __expf(m - m2), p = m2 == -INFINITY ? 0.f : __expf(s - m2);
-        l = l * keep + p;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 f = Pair16<T>::unpack(reinterpret_cast<const unsigned*>(a.v + v_at)[w * 32 + lane]);
-            o[2 * w] = o[2 * w] * keep + p * f.x;
-            o[2 * w + 1] = o[2 * w + 1] * keep + p * f.y;
-        }
-        m = m2;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-        reinterpret_cast<unsigned*>(a.out + (static_cast<long long>(r) * a.n_heads + h) * HD)[w * 32 + lane] = Pair16<T>::pack(o[2 * w] * inv, o[2 * w + 1] * inv);
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    uint4 v;
+    v.x = Pair16<T>::pack(o[0] * inv, o[1] * inv);
+    v.y = Pair16<T>::pack(o[2] * inv, o[3] * inv);
+    v.z = Pair16<T>::pack(o[4] * inv, o[5] * inv);
+    v.w = Pair16<T>::pack(o[6] * inv, o[7] * inv);
+    *reinterpret_cast<uint4*>(p.out + (static_cast<long long>(c.row + token) * p.n_heads + c.head + head) * HD + col) = v;
+}
+
+int launch_join(const EptqAttention& a, const AttentionPlan& plan, const AttentionArgs& p, cudaStream_t stream) {
+    const dim3 grid(plan.shares, plan.tile_rows / kJoinRows);
+    const int threads = kJoinRows * a.head_dim / 8;
+    if (a.dtype == EPTQ_FP16)
+        return a.head_dim == 128 ? launch_dependent(attention_join_kernel<__half, 128>, grid, threads, 0, stream, p)
+                                 : launch_dependent(attention_join_kernel<__half, 64>, grid, threads, 0, stream, p);
+    return a.head_dim == 128 ? launch_dependent(attention_join_kernel<__nv_bfloat16, 128>, grid, threads, 0, stream, p)
+                             : launch_dependent(attention_join_kernel<__nv_bfloat16, 64>, grid, threads, 0, stream, p);
 }
 
 int check(const EptqAttention& a) {
@@ -88,11 +93,27 @@ int check(const EptqAttention& a) {
                   a.table_stride < a.table_width)) return EPTQ_ERR_SHAPE;
     const int64_t kv_row = static_cast<int64_t>(a.n_kv_heads) * a.head_dim * (paged ? a.page_size : 1);
     if (a.q_stride < static_cast<int64_t>(a.n_heads) * a.head_dim || a.k_stride < kv_row || a.v_stride < kv_row) return EPTQ_ERR_SHAPE;
-    if (a.rows > 0 && a.batch > 0 && (a.q == nullptr || a.out == nullptr || a.cu_rows == nullptr || (paged && (a.kv_lens == nullptr || (a.tables == nullptr && a.table_width > 0))) ||
+    if (a.rows > 0 && a.batch > 0 && (a.q == nullptr || a.out == nullptr || a.cu_rows == nullptr ||
+                                      (paged && (a.kv_lens == nullptr || (a.tables == nullptr && a.table_width > 0))) ||
                                       ((!paged || a.n_pages > 0) && (a.k == nullptr || a.v == nullptr)))) return EPTQ_ERR_NULL;
     if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) || ((a.q_stride | a.k_stride | a.v_stride) % 8) != 0)
         return EPTQ_ERR_ALIGN;
     return EPTQ_OK;
+}
+
+// Rows of one key/value head of a request from which the tensor-core kernel takes a paged call.
+constexpr int kTensorRows = 32;
+
+bool on_tensor_cores(const EptqAttention& a) {
+    return a.page_size == 0 || static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > kTensorRows;
+}
+
+AttentionPlan plan_of(const EptqAttention& a) { return on_tensor_cores(a) ? attention_tcgen05_plan(a) : attention_rows_plan(a); }
+
+size_t cut_tile_bytes(const AttentionPlan& plan) { return (plan.shares * sizeof(CutTile) + 255) / 256 * 256; }
+
+size_t bytes_of(const EptqAttention& a, const AttentionPlan& plan) {
+    return plan.may_cut ? cut_tile_bytes(plan) + 2 * plan.shares * piece_floats(plan.tile_rows, a.head_dim) * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -100,28 +121,37 @@ int check(const EptqAttention& a) {
 
 using namespace eptq;
 
-// Rows of one key/value head of a request from which the tensor-core kernel takes a paged call.
-constexpr int kTensorRows = 32;
-
-static bool on_tensor_cores(const EptqAttention& a) {
-    if (a.page_size == 0) return true;
-    return a.n_pages > 0 && static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > kTensorRows;
-}
-
 extern "C" size_t eptq_ragged_attention_workspace_bytes(const EptqAttention* a) {
-    return a == nullptr || check(*a) != EPTQ_OK || !on_tensor_cores(*a) ? 0 : attention_tcgen05_bytes(*a);
+    return a == nullptr || check(*a) != EPTQ_OK ? 0 : bytes_of(*a, plan_of(*a));
 }
 
-extern "C" int eptq_ragged_attention(const EptqAttention* a, void* workspace, size_t workspace_bytes, void* stream) {
-    if (a == nullptr) return EPTQ_ERR_NULL;
-    if (const int st = check(*a); st != EPTQ_OK) return st;
-    if (a->rows == 0 || a->batch == 0) return EPTQ_OK;
-    if (on_tensor_cores(*a)) return launch_attention_tcgen05(*a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
-    const long long blocks = (static_cast<long long>(a->rows) * a->n_heads + kSimpleWarps - 1) / kSimpleWarps;
-    if (blocks > 2147483647LL) return EPTQ_ERR_SHAPE;
-    auto* kernel = a->dtype == EPTQ_FP16 ? (a->head_dim == 128 ? ragged_attention_simple_kernel<__half, 128> : ragged_attention_simple_kernel<__half, 64>)
-                                         : (a->head_dim == 128 ? ragged_attention_simple_kernel<__nv_bfloat16, 128> : ragged_attention_simple_kernel<__nv_bfloat16, 64>);
-    kernel<<<static_cast<unsigned>(blocks), kSimpleWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(*a);
-    count_launch(EPTQ_KERNEL_OTHER);
-    return cudaGetLastError() == cudaSuccess ? EPTQ_OK : EPTQ_ERR_LAUNCH;
+extern "C" int eptq_ragged_attention(const EptqAttention* args, void* workspace, size_t workspace_bytes, void* stream) {
+    if (args == nullptr) return EPTQ_ERR_NULL;
+    const EptqAttention& a = *args;
+    if (const int st = check(a); st != EPTQ_OK) return st;
+    if (a.rows == 0 || a.batch == 0) return EPTQ_OK;
+    const AttentionPlan plan = plan_of(a);
+    if (plan.may_cut && (workspace == nullptr || workspace_bytes < bytes_of(a, plan))) return EPTQ_ERR_WORKSPACE;
+    if (plan.may_cut && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return EPTQ_ERR_ALIGN;
+    int dev = 0;
+    if (attention_map_encoder() == nullptr || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return EPTQ_ERR_LAUNCH;
+    AttentionArgs p = {};
+    p.tables = a.tables; p.kv_lens = a.kv_lens; p.cu_rows = a.cu_rows;
+    p.q = a.q; p.q_stride = a.q_stride;
+    p.out = a.out; p.status = a.status;
+    p.cut_tiles = plan.may_cut ? static_cast<CutTile*>(workspace) : nullptr;
+    p.partial = plan.may_cut ? reinterpret_cast<float*>(static_cast<char*>(workspace) + cut_tile_bytes(plan)) : nullptr;
+    p.tile_rows = plan.tile_rows;
+    p.table_width = a.n_pages > 0 ? a.table_width : 0;           // no pages: no keys
+    p.table_stride = a.table_stride;
+    p.table_keys = static_cast<long long>(p.table_width) * a.page_size;
+    p.rows = a.rows; p.batch = a.batch; p.n_heads = a.n_heads;
+    p.kv_group = a.n_heads / a.n_kv_heads;
+    p.page_size = a.page_size; p.n_pages = a.n_pages;
+    // A scale of zero stays a step above it: masked scores are -infinity and must stay so.
+    p.scale_log2 = a.scale == 0.f ? 1e-30f : (a.scale < 0.f ? -a.scale : a.scale) * kLog2e;
+    p.negative = a.scale < 0.f;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int status = on_tensor_cores(a) ? launch_attention_tcgen05(a, p, dev, st) : launch_attention_rows(a, p, dev, st);
+    return status != EPTQ_OK || !plan.may_cut ? status : launch_join(a, plan, p, st);
 }
