@@ -76,7 +76,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
 def _build_host(force: bool, verbose: bool) -> None:
     from ._lib import host_path
     srcs, path = sorted((CSRC / "host").glob("*.cpp")), host_path()
-    if not force and not _newer(srcs + [HEADER], path):
+    if not force and not _newer(srcs + sorted((CSRC / "host").glob("*.hpp")) + [HEADER], path):
         return
     import sysconfig
 

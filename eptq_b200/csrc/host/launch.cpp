@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../../include/eptq_b200.h"
+#include "scratch.hpp"
 
 namespace {
 
@@ -116,6 +117,8 @@ std::vector<std::pair<int, at::Tensor>>& kept_scratch() {
     return *v;
 }
 
+}  // namespace
+
 at::Tensor scratch_for(int device, const c10::cuda::CUDAStream& stream, size_t bytes) {
     Scratch& s = scratch_map()[{device, static_cast<int64_t>(reinterpret_cast<intptr_t>(stream.stream()))}];
     if (!s.t.defined() || static_cast<size_t>(s.t.numel()) < bytes) {
@@ -133,6 +136,8 @@ at::Tensor scratch_for(int device, const c10::cuda::CUDAStream& stream, size_t b
     }
     return s.t;
 }
+
+namespace {
 
 bool fail(int status, const char* what) {
     PyErr_Format(PyExc_RuntimeError, "%s: %s (eptq status %d)", what, eptq_strerror(status), status);
@@ -384,4 +389,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_eptq_host", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__eptq_host(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__eptq_host(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddFunctions(m, paged_methods) != 0) Py_CLEAR(m);
+    return m;
+}
