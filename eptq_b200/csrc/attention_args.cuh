@@ -78,6 +78,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatil
 __device__ __forceinline__ bool warp_wait(unsigned bar, unsigned parity, volatile int* stop) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop));
 }
+// One lane of a converged warp.  Unlike `lane == 0` it tells the compiler that one thread runs what follows, which the
+// instructions that take uniform registers (tcgen05.mma, TMA) need: a loop over the active lanes around each of them cost
+// 195 cycles an MMA of 64.
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -109,6 +117,8 @@ struct ShareScratch {
     long long sums[kThreads / 32];
     long long before[2];         // blocks before the request that holds the share's begin and its end
     int request[2];
+    long long cut[2];
+    Place at;
 };
 
 // Sums the blocks of all requests, kPer requests a thread at a time, and finds the requests that hold the share's ends.
@@ -168,23 +178,37 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, in
         if (p.batch <= kThreads * kPer) break;                      // one chunk: both passes in one
     }
     __syncthreads();
-    long long cut[2];
-    for (int e = 0; e < 2; ++e) {
-        cut[e] = all;
-        if (ends[e] >= all) continue;
-        const int b = sh.request[e];
-        Place at = place_of(load_request(p, b), tile, kb, ends[e] - sh.before[e]);
-        const int step = moved(at, rule);
-        cut[e] = ends[e] + step;
-        if (e == 0) {
-            share.request = b;
-            at.block += step;
-            if (at.block == at.blocks) { at.block = 0; ++at.tile; }
-            share.at = at;
+    if (warp < 2) {                                                 // one warp for each end
+        const long long end = warp == 0 ? ends[0] : ends[1];
+        long long cut = all;
+        if (end < all) {
+            const Request r = load_request(p, sh.request[warp]);
+            // 32 tiles looked at in each round: the sums before a tile take a few divisions
+            Place at = place_of(r, tile, kb, end - sh.before[warp], [&](int lo, int hi, long long y) {
+                while (lo < hi) {
+                    const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
+                    const bool begins = i <= hi && blocks_before(r, tile, kb, i) <= y;
+                    const int n = __popc(__ballot_sync(0xffffffffu, begins));      // beginnings rise: the first n lanes
+                    lo += n * step;
+                    hi = min(hi, lo + step - 1);
+                }
+                return lo;
+            });
+            const int step = moved(at, rule);
+            cut = end + step;
+            if (warp == 0 && lane == 0) {
+                at.block += step;
+                if (at.block == at.blocks) { at.block = 0; ++at.tile; }
+                sh.at = at;
+            }
         }
+        if (lane == 0) sh.cut[warp] = cut;
     }
-    share.begin = cut[0];
-    share.end = cut[1];
+    __syncthreads();
+    share.request = sh.request[0];
+    share.at = sh.at;
+    share.begin = sh.cut[0];
+    share.end = sh.cut[1];
     return share;
 }
 

@@ -50,21 +50,38 @@ EPTQ_HD int blocks_of(const Request& r, int tile, int kb, int i) {
     return keys <= kb ? 1 : static_cast<int>((keys + kb - 1) / kb);
 }
 
-// sum of floor((a i + b) / m) for i = 0 .. n-1, a, b >= 0: the usual exchange of the axes under the line
-// (Euclid's algorithm on a and m).
+// sum of floor((a i + b) / m) for i = 0 .. n-1, a, b >= 0: the usual exchange of the axes under the line (Euclid's
+// algorithm on a and m).  Needs a n + b < 2^32 once a and b are reduced by m, which holds here: a is at most the tokens of a
+// tile, n the tiles of a request.
 EPTQ_HD long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-    long long sum = 0;
+    // the first step apart: its m is a constant power of two of the caller, and where it divides a the sum is done
+    long long sum = static_cast<long long>(n) * (n - 1) / 2 * (a / m) + static_cast<long long>(n) * (b / m);
+    a %= m;
+    b %= m;
+    const unsigned top0 = a * n + b;
+    if (n == 0 || top0 < m) return sum;
+    n = top0 / m;
+    b = top0 % m;
+    {
+        const unsigned t = m; m = a; a = t;
+    }
     while (n > 0) {
         sum += static_cast<long long>(n) * (n - 1) / 2 * (a / m) + static_cast<long long>(n) * (b / m);
         a %= m;
         b %= m;
-        const unsigned long long top = static_cast<unsigned long long>(a) * n + b;
+        const unsigned top = a * n + b;
         if (top < m) break;
-        n = static_cast<unsigned>(top / m);
-        b = static_cast<unsigned>(top % m);
+        n = top / m;
+        b = top % m;
         const unsigned t = m; m = a; a = t;
     }
     return sum;
+}
+
+// 64-bit division is a long routine on the device; nearly all quotients here are of 32-bit values.
+EPTQ_HD long long quotient(long long x, long long y) {
+    if (((x | y) >> 32) == 0) return static_cast<unsigned>(x) / static_cast<unsigned>(y);
+    return x / y;
 }
 
 // Blocks of the row tiles before tile i, i <= tiles_of.
@@ -87,26 +104,23 @@ struct Place {
     int blocks;                // of that row tile
 };
 
-// x = blocks of the request before the place, 0 <= x < groups * blocks_before(all tiles).
-EPTQ_HD Place place_of(const Request& r, int tile, int kb, long long x) {
+// x = blocks of the request before the place, 0 <= x < groups * blocks_before(all tiles).  `last_tile_at(lo, hi, y)` gives the
+// last tile of lo .. hi that begins at or before y.
+template <typename Search>
+EPTQ_HD Place place_of(const Request& r, int tile, int kb, long long x, const Search& last_tile_at) {
     const int tiles = tiles_of(r, tile);
     const long long per_group = blocks_before(r, tile, kb, tiles);
     Place p;
-    p.group = static_cast<int>(x / per_group);
+    p.group = static_cast<int>(quotient(x, per_group));
     const long long y = x - p.group * per_group;
-    int lo = 0, hi = tiles - 1;                       // the last tile that begins at or before y
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (blocks_before(r, tile, kb, mid) <= y) lo = mid; else hi = mid - 1;
-    }
-    p.tile = lo;
-    p.block = static_cast<int>(y - blocks_before(r, tile, kb, lo));
-    p.blocks = blocks_of(r, tile, kb, lo);
+    p.tile = last_tile_at(0, tiles - 1, y);
+    p.block = static_cast<int>(y - blocks_before(r, tile, kb, p.tile));
+    p.blocks = blocks_of(r, tile, kb, p.tile);
     return p;
 }
 
 EPTQ_HD long long share_of(long long all_blocks, int n_shares, const CutRule& rule) {
-    const long long u = (all_blocks + n_shares - 1) / n_shares;
+    const long long u = quotient(all_blocks + n_shares - 1, n_shares);
     return u < rule.share ? rule.share : u;
 }
 
@@ -121,7 +135,7 @@ EPTQ_HD int moved(const Place& p, const CutRule& rule) {
 
 // The last share that holds blocks of a cut tile which ends at `tile_end` in the sequence.
 EPTQ_HD int last_share(long long tile_end, long long share, const CutRule& rule) {
-    return static_cast<int>((tile_end - rule.near + share - 1) / share) - 1;
+    return static_cast<int>(quotient(tile_end - rule.near + share - 1, share)) - 1;
 }
 
 }  // namespace eptq

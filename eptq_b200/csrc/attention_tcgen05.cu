@@ -7,7 +7,7 @@
 // head), so a block of keys is read once for all of them and few tokens fill the rows.  Blocks of 128 keys.
 //
 //   warp 0      walks this block's share of the work (attention_schedule.cuh), tells the others its items through a small
-//               ring, loads Q once per item and K and V by TMA (128-byte swizzle) into a ring of 128-key slots.
+//               ring, loads Q once per item and K by TMA (128-byte swizzle) into a ring of 128-key slots; warp 2 loads V.
 //   warp 1      issues the tcgen05.mma: S = Q K^T (M 128, N 128) into TMEM, and O += P V with P read from TMEM where S was
 //               and V from shared memory as it lies (keys along K, head columns contiguous).  S of one half is formed while
 //               the other half's softmax runs.
@@ -35,14 +35,14 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kKeyBlock = 128;
 constexpr int kItems = 4;                      // ring of items
-constexpr int kMaxSlots = 10;
+constexpr int kMaxSlots = 5;
 constexpr int kKeysSeen = 16;                  // ring of per-block page flags
 
-// Q: two halves of 128 rows; K and V: slots of 128 keys; each in head_dim / 64 boxes of 128-byte rows.
+// Q: two halves of 128 rows; K and V: rings of slots of 128 keys; each in head_dim / 64 boxes of 128-byte rows.
 __host__ __device__ constexpr int tile_bytes(int hd) { return 128 * hd * 2; }
-__host__ __device__ constexpr int slots(int hd) { return hd == 128 ? 5 : 10; }
-__host__ __device__ constexpr int smem_bytes(int hd) { return (2 + slots(hd)) * tile_bytes(hd) + 1024; }
-static_assert(slots(64) <= kMaxSlots && slots(128) <= kMaxSlots, "barrier array");
+__host__ __device__ constexpr int k_slots(int hd) { return hd == 128 ? 3 : 5; }
+__host__ __device__ constexpr int v_slots(int hd) { return hd == 128 ? 2 : 5; }
+__host__ __device__ constexpr int smem_bytes(int hd) { return (2 + k_slots(hd) + v_slots(hd)) * tile_bytes(hd) + 1024; }
 
 __device__ __forceinline__ void commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
@@ -100,15 +100,71 @@ __device__ __forceinline__ void tmem_st32(unsigned addr, const unsigned* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // An item and the blocks of keys that either half of its rows sees.
 struct HalvedItem {
     Item it;
     int count[2];
+    int first;                             // the request's first row
 };
 
+// The page table's columns column .. column + 31 of one request, one per lane.
+struct PageRow {
+    int column, id;
+
+    // Pages of `keys` keys from key0 on: their number, and in lane i the i-th one's id (n_pages where it is outside the cache,
+    // which reads as zeros).
+    __device__ __forceinline__ int fetch(const AttentionArgs& p, int request, int key0, int keys, int lane, int& page) {
+        const int shift = 31 - __clz(p.page_size), at = key0 >> shift, n = (max(0, keys) + p.page_size - 1) >> shift;
+        if (column < 0 || at + n > column + 32) {
+            column = at;
+            id = at + lane < p.table_width ? __ldg(p.tables + request * p.table_stride + at + lane) : -1;
+        }
+        page = __shfl_sync(0xffffffffu, id, (at - column + lane) & 31);
+        if (page < 0 || page >= p.n_pages) page = p.n_pages;
+        return n;
+    }
+};
+
+// One block of keys or values into a slot, by a whole warp.
+template <int HD, bool PAGED>
+__device__ __forceinline__ void load_keys(const AttentionArgs& p, const CUtensorMap* map, unsigned dst, unsigned bar, int row, int head, int n_pages, int page) {
+    constexpr int kBoxBytes = 128 * 64 * 2;
+    if (PAGED) {
+        if (elect_one()) mbar_arrive_expect_tx(bar, n_pages * p.page_size * HD * 2);
+        for (int i = 0; i < n_pages; ++i) {
+            const int id = __shfl_sync(0xffffffffu, page, i);
+            if (elect_one()) {
+#pragma unroll
+                for (int x = 0; x < HD / 64; ++x) tma_4d(dst + x * kBoxBytes + i * p.page_size * 128, map, x * 64, 0, head, id, bar);
+            }
+        }
+    } else if (elect_one()) {
+        mbar_arrive_expect_tx(bar, tile_bytes(HD));
+#pragma unroll
+        for (int x = 0; x < HD / 64; ++x) tma_3d(dst + x * kBoxBytes, map, x * 64, head, row, bar);
+    }
+    __syncwarp();
+}
+
 struct Shared {
-    unsigned long long q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
-    unsigned long long kv_full[kMaxSlots], kv_empty[kMaxSlots], item_full[kItems], item_empty[kItems];
+    unsigned long long q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2];
+    unsigned long long k_full[kMaxSlots], k_empty[kMaxSlots], v_full[kMaxSlots], v_empty[kMaxSlots], item_full[kItems], item_empty[kItems];
     HalvedItem items[kItems];
     ShareScratch<kThreads> share;
     unsigned lost[kKeysSeen];              // 16-key groups of a block that are on no page of the cache
@@ -123,10 +179,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Shared sh;
     constexpr int kBoxes = HD / 64;
-    constexpr int kTile = tile_bytes(HD), kBox = 128 * 64 * 2, kSlots = slots(HD);
+    constexpr int kTile = tile_bytes(HD), kBox = 128 * 64 * 2, kKSlots = k_slots(HD), kVSlots = v_slots(HD);
     constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
     unsigned char* const tiles = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned char* const k_tiles = tiles + 2 * kTile;
+    unsigned char* const v_tiles = k_tiles + kKSlots * kTile;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int tile_tokens = 2 * p.tokens_per_half;
 
     if (tid == 0) {
@@ -134,17 +192,20 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(smem_u32(&sh.q_full[h]), 1);
             mbar_init(smem_u32(&sh.q_empty[h]), 1);
             mbar_init(smem_u32(&sh.s_full[h]), 1);
-            mbar_init(smem_u32(&sh.p_full[h]), 4);
+            mbar_init(smem_u32(&sh.p_full[h][0]), 4);
+            mbar_init(smem_u32(&sh.p_full[h][1]), 4);
             mbar_init(smem_u32(&sh.o_full[h]), 1);
             mbar_init(smem_u32(&sh.o_empty[h]), 4);
         }
-        for (int s = 0; s < kSlots; ++s) {
-            mbar_init(smem_u32(&sh.kv_full[s]), 1);
-            mbar_init(smem_u32(&sh.kv_empty[s]), 1);
+        for (int s = 0; s < kMaxSlots; ++s) {
+            mbar_init(smem_u32(&sh.k_full[s]), 1);
+            mbar_init(smem_u32(&sh.k_empty[s]), 1);
+            mbar_init(smem_u32(&sh.v_full[s]), 1);
+            mbar_init(smem_u32(&sh.v_empty[s]), 1);
         }
         for (int s = 0; s < kItems; ++s) {
             mbar_init(smem_u32(&sh.item_full[s]), 1);
-            mbar_init(smem_u32(&sh.item_empty[s]), 9);
+            mbar_init(smem_u32(&sh.item_empty[s]), 10);
         }
         sh.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -174,20 +235,21 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
-            // ---------------- items and loads
+            // ---------------- items, Q and K
             ShareWalk walk;
             walk.start(p, share);
-            unsigned kv_seq = 0, n_items = 0, q_count[2] = {0, 0}, block_seq = 0;
+            unsigned k_seq = 0, n_items = 0, q_count[2] = {0, 0}, block_seq = 0;
             bool cut_written = false;
+            PageRow pages;
+            HalvedItem hit;
+            Item& it = hit.it;
+            bool more = walk.next(p, tile_tokens, kKeyBlock, rule, it);
             for (;;) {
-                HalvedItem hit;
-                Item& it = hit.it;
-                const bool more = walk.next(p, tile_tokens, kKeyBlock, rule, it);
                 const int ring = n_items % kItems;
                 ok = warp_wait(smem_u32(&sh.item_empty[ring]), ((n_items / kItems) & 1u) ^ 1u, &sh.stop);
                 if (!ok) break;
                 if (!more) {
-                    if (lane == 0) {
+                    if (elect_one()) {
                         sh.items[ring].it.request = -1;
                         mbar_arrive(smem_u32(&sh.item_full[ring]));
                     }
@@ -198,90 +260,104 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int need0 = keys0 <= kKeyBlock ? 1 : (keys0 + kKeyBlock - 1) / kKeyBlock;
                 hit.count[0] = max(0, min(it.blocks, need0 - it.block));
                 hit.count[1] = it.tokens > p.tokens_per_half ? it.blocks : 0;
-                if (lane == 0) {
+                hit.first = walk.r.first;
+                if (elect_one()) {
                     sh.items[ring] = hit;
                     mbar_arrive(smem_u32(&sh.item_full[ring]));
-                    if (it.of > 0) {
-                        write_cut_tile(p, it);
-                        cut_written = true;
-                    }
+                    if (it.of > 0) write_cut_tile(p, it);
                 }
+                cut_written |= it.of > 0;
                 ++n_items;
-                for (int h = 0; h < 2 && ok; ++h) {
-                    if (hit.count[h] == 0) continue;
-                    ok = warp_wait(smem_u32(&sh.q_empty[h]), (q_count[h] & 1u) ^ 1u, &sh.stop);
-                    if (!ok) break;
+                const int kv_head = it.head / p.kv_group;
+                pages.column = -1;
+                auto load_q = [&](int h) {
+                    if (hit.count[h] == 0) return true;
+                    if (!warp_wait(smem_u32(&sh.q_empty[h]), (q_count[h] & 1u) ^ 1u, &sh.stop)) return false;
                     ++q_count[h];
-                    if (lane == 0) {
+                    if (elect_one()) {
                         const unsigned bar = smem_u32(&sh.q_full[h]);
                         mbar_arrive_expect_tx(bar, p.heads_per_tile * p.tokens_per_half * HD * 2);
+#pragma unroll
                         for (int x = 0; x < kBoxes; ++x)
                             tma_3d(smem_u32(tiles + h * kTile + x * kBox), &map_q, x * 64, it.head, it.row + h * p.tokens_per_half, bar);
                     }
-                }
-                const int kv_head = it.head / p.kv_group;
-                int table_at = -1, page_id = 0;                    // table columns table_at .. table_at + 31, one per lane
+                    __syncwarp();
+                    return true;
+                };
+                ok = load_q(0);
                 for (int j = 0; j < it.blocks && ok; ++j) {
                     const int key0 = (it.block + j) * kKeyBlock;
-                    int pages = 0, page = 0;
-                    unsigned lost = 0;
+                    int n_pages = 0, page = 0;
                     if (PAGED) {
-                        // this block's pages: lane i holds page i
-                        pages = (max(0, min(kKeyBlock, it.keys - key0)) + p.page_size - 1) / p.page_size;
-                        const int col = key0 / p.page_size;
-                        if (table_at < 0 || col < table_at || col + pages > table_at + 32) {
-                            table_at = col;
-                            page_id = col + lane < p.table_width ? __ldg(p.tables + it.request * p.table_stride + col + lane) : -1;
-                        }
-                        page = __shfl_sync(0xffffffffu, page_id, (col - table_at + lane) & 31);
-                        const bool gone = lane < pages && (page < 0 || page >= p.n_pages);
-                        if (gone) page = p.n_pages;                // outside: reads as zeros
-                        const unsigned bad = __ballot_sync(0xffffffffu, gone);
+                        n_pages = pages.fetch(p, it.request, key0, min(kKeyBlock, it.keys - key0), lane, page);
+                        const unsigned bad = __ballot_sync(0xffffffffu, lane < n_pages && page == p.n_pages);
+                        unsigned lost = 0;
                         if (bad) {
                             const int per = p.page_size / 16;
                             for (int i = 0; i < 8; ++i)
                                 if ((bad >> (i / per)) & 1u) lost |= 1u << i;
                         }
-                        if (lane == 0) sh.lost[block_seq % kKeysSeen] = lost;
+                        if (elect_one()) sh.lost[block_seq % kKeysSeen] = lost;
                         ++block_seq;
                     }
-                    for (int kv = 0; kv < 2; ++kv, ++kv_seq) {
-                        const int s = kv_seq % kSlots;
-                        ok = warp_wait(smem_u32(&sh.kv_empty[s]), ((kv_seq / kSlots) & 1u) ^ 1u, &sh.stop);
-                        if (!ok) break;
-                        const unsigned bar = smem_u32(&sh.kv_full[s]);
-                        const unsigned dst = smem_u32(tiles + (2 + s) * kTile);
-                        const CUtensorMap* map = kv ? &map_v : &map_k;
-                        if (PAGED) {
-                            if (lane == 0) mbar_arrive_expect_tx(bar, pages * p.page_size * HD * 2);
-                            __syncwarp();
-                            if (lane < pages)
-                                for (int x = 0; x < kBoxes; ++x)
-                                    tma_4d(dst + x * kBox + lane * p.page_size * 128, map, x * 64, 0, kv_head, page, bar);
-                        } else if (lane == 0) {
-                            mbar_arrive_expect_tx(bar, kTile);
-                            for (int x = 0; x < kBoxes; ++x)
-                                tma_3d(dst + x * kBox, map, x * 64, kv_head, walk.r.first + key0, bar);
-                        }
-                    }
+                    const int s = k_seq % kKSlots;
+                    ok = warp_wait(smem_u32(&sh.k_empty[s]), ((k_seq / kKSlots) & 1u) ^ 1u, &sh.stop);
+                    if (!ok) break;
+                    ++k_seq;
+                    load_keys<HD, PAGED>(p, &map_k, smem_u32(k_tiles + s * kTile), smem_u32(&sh.k_full[s]), hit.first + key0, kv_head, n_pages, page);
+                    if (j == 0) ok = load_q(1);
                 }
                 if (!ok) break;
+                more = walk.next(p, tile_tokens, kKeyBlock, rule, it);
             }
             if (lane == 0 && !cut_written && p.cut_tiles != nullptr) p.cut_tiles[blockIdx.x].of = 0;
             if (!ok) {
                 // copies still in flight write shared memory: wait for them before it is given up
-                __syncwarp();
                 volatile int never = 0;
                 for (int h = 0; h < 2; ++h)
-                    if (q_count[h] > 0) mbar_wait(smem_u32(&sh.q_full[h]), (q_count[h] - 1) & 1u, &never);
-                for (unsigned i = kv_seq > kSlots ? kv_seq - kSlots : 0; i < kv_seq; ++i)
-                    mbar_wait(smem_u32(&sh.kv_full[i % kSlots]), (i / kSlots) & 1u, &never);
+                    if (q_count[h] > 0) warp_wait(smem_u32(&sh.q_full[h]), (q_count[h] - 1) & 1u, &never);
+                for (unsigned i = k_seq > kKSlots ? k_seq - kKSlots : 0; i < k_seq; ++i)
+                    warp_wait(smem_u32(&sh.k_full[i % kKSlots]), (i / kKSlots) & 1u, &never);
+            }
+        } else if (warp == 2) {
+            // ---------------- V
+            unsigned v_seq = 0, n_items = 0;
+            PageRow pages;
+            while (ok) {
+                const int ring = n_items % kItems;
+                ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
+                if (!ok) break;
+                const Item it = sh.items[ring].it;
+                const int first = sh.items[ring].first;
+                if (it.request < 0) break;
+                ++n_items;
+                const int kv_head = it.head / p.kv_group;
+                pages.column = -1;
+                for (int j = 0; j < it.blocks && ok; ++j) {
+                    const int key0 = (it.block + j) * kKeyBlock;
+                    int n_pages = 0, page = 0;
+                    if (PAGED) n_pages = pages.fetch(p, it.request, key0, min(kKeyBlock, it.keys - key0), lane, page);
+                    const int s = v_seq % kVSlots;
+                    ok = warp_wait(smem_u32(&sh.v_empty[s]), ((v_seq / kVSlots) & 1u) ^ 1u, &sh.stop);
+                    if (!ok) break;
+                    ++v_seq;
+                    load_keys<HD, PAGED>(p, &map_v, smem_u32(v_tiles + s * kTile), smem_u32(&sh.v_full[s]), first + key0, kv_head, n_pages, page);
+                }
+                __syncwarp();
+                if (elect_one()) mbar_arrive(smem_u32(&sh.item_empty[ring]));
+            }
+            if (!ok) {
+                volatile int never = 0;
+                for (unsigned i = v_seq > kVSlots ? v_seq - kVSlots : 0; i < v_seq; ++i)
+                    warp_wait(smem_u32(&sh.v_full[i % kVSlots]), (i / kVSlots) & 1u, &never);
             }
         } else if (warp == 1) {
             // ---------------- MMA
             const uint32_t qk = instr_desc(kKeyBlock, kBf16, false, p.negative != 0);
-            const uint32_t pv = instr_desc(HD, kBf16, true, false);
-            unsigned kv_seq = 0, n_items = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0}, o_count[2] = {0, 0};
+            constexpr uint32_t pv = instr_desc(HD, kBf16, true, false);
+            const uint64_t q_desc = desc_sw128(smem_u32(tiles), 16), k_desc = desc_sw128(smem_u32(k_tiles), 16);
+            const uint64_t v_desc = desc_sw128(smem_u32(v_tiles), kBox);
+            unsigned k_seq = 0, v_seq = 0, n_items = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0}, o_count[2] = {0, 0};
             while (ok) {
                 const int ring = n_items % kItems;
                 ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
@@ -293,20 +369,20 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (request < 0) break;
                 ++n_items;
                 for (int j = 0; j <= blocks && ok; ++j) {
-                    const unsigned k_seq = kv_seq + 2 * j, v_seq = kv_seq + 2 * j - 1;
-                    const int k_slot = k_seq % kSlots, v_slot = v_seq % kSlots;
+                    const int k_slot = k_seq % kKSlots, v_slot = v_seq % kVSlots;        // of K(j) and V(j - 1)
                     bool k_here = false, v_here = false;
-                    for (int h = 0; h < 2 && ok; ++h) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
                         const unsigned s_at = tmem + h * 128, o_at = tmem + 256 + h * HD;
                         if (j > 0 && j - 1 < count[h]) {
                             const int live = min(kKeyBlock, max(0, keys - (j - 1) * kKeyBlock));
                             if (!v_here) {
-                                ok = warp_wait(smem_u32(&sh.kv_full[v_slot]), (v_seq / kSlots) & 1u, &sh.stop);
+                                ok = warp_wait(smem_u32(&sh.v_full[v_slot]), (v_seq / kVSlots) & 1u, &sh.stop);
                                 if (!ok) break;
                                 v_here = true;
                                 if (live & 15) {                  // clear the rest of the last 16 keys
                                     const int gone = 16 - (live & 15);
-                                    unsigned char* const v = tiles + (2 + v_slot) * kTile + live * 128;
+                                    unsigned char* const v = v_tiles + v_slot * kTile + live * 128;
                                     for (int i = lane; i < gone * 8 * kBoxes; i += 32)
                                         *reinterpret_cast<uint4*>(v + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
                                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -318,22 +394,32 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                                 if (!ok) break;
                                 ++o_count[h];
                             }
-                            ok = warp_wait(smem_u32(&sh.p_full[h]), p_count[h] & 1u, &sh.stop);
+                            const uint64_t dv = v_desc + static_cast<uint64_t>((v_slot * kTile) >> 4);
+#pragma unroll
+                            for (int part = 0; part < 2; ++part) {      // P comes in two parts of 64 keys
+                                ok = warp_wait(smem_u32(&sh.p_full[h][part]), p_count[h] & 1u, &sh.stop);
+                                if (!ok) break;
+                                fence_after();
+                                if (elect_one()) {
+                                    if (live >= part * 64 + 64) {
+#pragma unroll
+                                        for (int k = part * 4; k < part * 4 + 4; ++k)
+                                            mma_tmem(o_at, s_at + k * 8, dv + ((k * 2048) >> 4), pv, j > 1 || k > 0);
+                                    } else {
+#pragma unroll 1
+                                        for (int k = part * 4; k * 16 < live; ++k)
+                                            mma_tmem(o_at, s_at + k * 8, dv + static_cast<uint64_t>((k * 2048) >> 4), pv, j > 1 || k > 0);
+                                    }
+                                    if (part == 1 && j == count[h]) commit(smem_u32(&sh.o_full[h]));
+                                }
+                                __syncwarp();
+                            }
                             if (!ok) break;
                             ++p_count[h];
-                            fence_after();
-                            if (lane == 0) {
-                                const uint64_t dv = desc_sw128(smem_u32(tiles + (2 + v_slot) * kTile), kBox);
-                                const int steps = (live + 15) >> 4;
-                                for (int k = 0; k < steps; ++k)
-                                    mma_tmem(o_at, s_at + k * 8, dv + static_cast<uint64_t>((k * 2048) >> 4), pv, j > 1 || k > 0);
-                                if (j == count[h]) commit(smem_u32(&sh.o_full[h]));
-                            }
-                            __syncwarp();
                         }
                         if (j < count[h]) {
                             if (!k_here) {
-                                ok = warp_wait(smem_u32(&sh.kv_full[k_slot]), (k_seq / kSlots) & 1u, &sh.stop);
+                                ok = warp_wait(smem_u32(&sh.k_full[k_slot]), (k_seq / kKSlots) & 1u, &sh.stop);
                                 if (!ok) break;
                                 k_here = true;
                             }
@@ -343,13 +429,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                                 ++q_count[h];
                             }
                             fence_after();
-                            if (lane == 0) {
-                                for (int x = 0; x < kBoxes; ++x) {
-                                    const uint64_t dq = desc_sw128(smem_u32(tiles + h * kTile + x * kBox), 16);
-                                    const uint64_t dk = desc_sw128(smem_u32(tiles + (2 + k_slot) * kTile + x * kBox), 16);
+                            if (elect_one()) {
+                                const uint64_t dq = q_desc + ((h * kTile) >> 4), dk = k_desc + static_cast<uint64_t>((k_slot * kTile) >> 4);
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k)
-                                        mma_smem(s_at, dq + static_cast<uint64_t>((k * 32) >> 4), dk + static_cast<uint64_t>((k * 32) >> 4), qk, x > 0 || k > 0);
+                                for (int k = 0; k < HD / 16; ++k) {
+                                    const uint64_t at = ((k >> 2) * kBox + (k & 3) * 32) >> 4;
+                                    mma_smem(s_at, dq + at, dk + at, qk, k > 0);
                                 }
                                 commit(smem_u32(&sh.s_full[h]));
                                 if (j == count[h] - 1) commit(smem_u32(&sh.q_empty[h]));
@@ -358,15 +443,16 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                     if (!ok) break;
-                    if (lane == 0) {
-                        if (j > 0) commit(smem_u32(&sh.kv_empty[v_slot]));
-                        if (j < blocks) commit(smem_u32(&sh.kv_empty[k_slot]));
+                    if (elect_one()) {
+                        if (j > 0) commit(smem_u32(&sh.v_empty[v_slot]));
+                        if (j < blocks) commit(smem_u32(&sh.k_empty[k_slot]));
                     }
                     __syncwarp();
+                    if (j > 0) ++v_seq;
+                    if (j < blocks) ++k_seq;
                 }
-                kv_seq += 2 * blocks;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.item_empty[ring]));
+                if (elect_one()) mbar_arrive(smem_u32(&sh.item_empty[ring]));
             }
         }
     } else {
@@ -407,9 +493,14 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     for (int i = 0; i < 128; ++i)
                         if (i >= allowed || (PAGED && ((lost >> (i / 16)) & 1u))) s[i] = -INFINITY;
                 }
-                float m = top;
+                float m8[8];                                    // eight chains: one would wait for itself 128 times
 #pragma unroll
-                for (int i = 0; i < 128; ++i) m = fmaxf(m, s[i]);
+                for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[i + 8]);
+#pragma unroll
+                for (int i = 16; i < 128; i += 16)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) m8[k] = fmaxf(fmaxf(m8[k], s[i + k]), s[i + k + 8]);
+                const float m = fmaxf(fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))), top);
                 // The exponents' reference moves only when it has to: on the first block that has keys, or by more than 2^8.
                 const bool first = top == -INFINITY;
                 const bool moves = first ? m > -INFINITY : (m - top) * p.scale_log2 > kRescaleAt;
@@ -431,25 +522,26 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                 }
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), bias2 = make_float2(-bias, -bias);
+                float2 part[4];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     unsigned w[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float a = exp2_approx(fmaf(s[c * 64 + 2 * i], p.scale_log2, -bias));
-                        const float b = exp2_approx(fmaf(s[c * 64 + 2 * i + 1], p.scale_log2, -bias));
-                        part[(2 * i) & 3] += a;
-                        part[(2 * i + 1) & 3] += b;
-                        w[i] = Pair16<T>::pack(a, b);
+                        float2 e = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, bias2);
+                        e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                        part[i & 3] = c == 0 && i < 4 ? e : add2(part[i & 3], e);
+                        w[i] = Pair16<T>::pack(e.x, e.y);
                     }
                     tmem_st32(s_at + c * 32, w);
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[h][c]));
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[h]));
+                const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+                sum += all.x + all.y;
             }
             block_seq += it.blocks;
             if (!ok) break;
@@ -517,7 +609,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
-constexpr CutRule kRule = {8, 2, 4};
+constexpr CutRule kRule = {8, 2, 1};
 template <typename T, int HD, bool PAGED>
 int run(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {
     static std::once_flag once[64];
