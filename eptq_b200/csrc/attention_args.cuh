@@ -33,7 +33,7 @@ struct AttentionArgs {
     int negative;                  // scale is below zero
 };
 
-// A piece of a cut tile: o [tile_rows][head_dim], then the exponent's reference and the sum of each row, fp32.  Rows whose
+// A piece of a cut tile: o [head_dim / 4][tile_rows][4], then the exponent's reference and the sum of each row, fp32.  Rows whose
 // sum is zero have no o.
 __host__ __device__ constexpr long long piece_floats(int rows, int hd) { return static_cast<long long>(rows) * (hd + 2); }
 
@@ -124,7 +124,7 @@ struct ShareScratch {
 // Sums the blocks of all requests, kPer requests a thread at a time, and finds the requests that hold the share's ends.
 // All threads of the block call it and get the same answer.
 template <int kThreads, int kPer>
-__device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, int kb, const CutRule& rule, ShareScratch<kThreads>& sh) {
+__device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, int kb, CutRule& rule, ShareScratch<kThreads>& sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, groups = p.n_heads / p.heads_per_tile;
     long long all = 0, ends[2] = {0, 0};
     Share share = {};

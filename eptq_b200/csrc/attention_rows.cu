@@ -54,7 +54,7 @@ __device__ __forceinline__ float quad_sum(float v) {
 template <typename T, int HD, int MT>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(MT))
 attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                      const __grid_constant__ AttentionArgs p, const CutRule rule) {
+                      const __grid_constant__ AttentionArgs p, CutRule rule) {
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(8) unsigned long long full[kWarps][stages(MT)];
     __shared__ ShareScratch<kThreads> share_scratch;
@@ -318,8 +318,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 *reinterpret_cast<uint4*>(p.out + (static_cast<long long>(it.row + token) * p.n_heads + it.head + row % p.heads_per_tile) * HD + col) = out;
             } else {
                 float* const piece = p.partial + it.slot * piece_floats(16 * MT, HD);
-                reinterpret_cast<float4*>(piece + row * HD + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(piece + row * HD + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                reinterpret_cast<float4*>(piece)[col / 4 * (16 * MT) + row] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4*>(piece)[(col / 4 + 1) * (16 * MT) + row] = make_float4(v[4], v[5], v[6], v[7]);
                 if (col == 0) {
                     piece[16 * MT * HD + row] = all == 0.f ? 0.f : high;
                     piece[16 * MT * HD + 16 * MT + row] = all;

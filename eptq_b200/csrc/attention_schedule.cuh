@@ -20,7 +20,7 @@ namespace eptq {
 
 struct CutRule {
     int least;     // a tile of at most this many blocks is not cut
-    int near;      // a cut this near an end of its tile moves there
+    int near;      // a cut this near an end of its tile moves there, where that is at most an eighth of a share
     int share;     // least blocks of a share
 };
 
@@ -48,6 +48,27 @@ EPTQ_HD int blocks_of(const Request& r, int tile, int kb, int i) {
     const long long rows = static_cast<long long>(i + 1) * tile < r.n ? static_cast<long long>(i + 1) * tile : r.n;
     const long long keys = r.past + rows;
     return keys <= kb ? 1 : static_cast<int>((keys + kb - 1) / kb);
+}
+
+EPTQ_HD int log2_of(unsigned power) {
+#ifdef __CUDA_ARCH__
+    return 31 - __clz(power);
+#else
+    return 31 - __builtin_clz(power);
+#endif
+}
+
+// sum of floor((a i + b) / m) for i = 0 .. n-1, b >= 0, a and m powers of two: shifts, no division.
+EPTQ_HD long long floor_sum_powers(unsigned n, unsigned m, unsigned a, unsigned b) {
+    const int am = log2_of(a), mm = log2_of(m);
+    if (am >= mm) return (static_cast<long long>(n) * (n - 1) / 2 << (am - mm)) + static_cast<long long>(n) * (b >> mm);
+    // floor((a i + b) / m) = floor((i + c) / d), c = floor(b / a), d = m / a: whole runs of d, then the rest of one
+    const int d = mm - am;
+    const unsigned c = b >> am, top = c + n;
+    const long long qt = top >> d, qc = c >> d;
+    const long long upto_top = (qt * (qt - 1) / 2 << d) + qt * (top & ((1u << d) - 1));
+    const long long upto_c = (qc * (qc - 1) / 2 << d) + qc * (c & ((1u << d) - 1));
+    return upto_top - upto_c;
 }
 
 // sum of floor((a i + b) / m) for i = 0 .. n-1, a, b >= 0: the usual exchange of the axes under the line (Euclid's
@@ -91,9 +112,10 @@ EPTQ_HD long long blocks_before(const Request& r, int tile, int kb, int i) {
     int z = r.past < 0 ? -r.past / tile : 0;                                      // tiles without keys: one block each
     if (z > full) z = full;
     long long sum = z;
-    if (full > z)
-        sum += floor_sum(static_cast<unsigned>(full - z), kb, static_cast<unsigned>(tile),
-                         static_cast<unsigned>(r.past + static_cast<long long>(z + 1) * tile + kb - 1));
+    if (full > z) {
+        const unsigned n = static_cast<unsigned>(full - z), b = static_cast<unsigned>(r.past + static_cast<long long>(z + 1) * tile + kb - 1);
+        sum += (tile & (tile - 1)) == 0 ? floor_sum_powers(n, kb, tile, b) : floor_sum(n, kb, tile, b);
+    }
     if (i > full) sum += blocks_of(r, tile, kb, i - 1);
     return sum;
 }
@@ -119,9 +141,10 @@ EPTQ_HD Place place_of(const Request& r, int tile, int kb, long long x, const Se
     return p;
 }
 
-EPTQ_HD long long share_of(long long all_blocks, int n_shares, const CutRule& rule) {
-    const long long u = quotient(all_blocks + n_shares - 1, n_shares);
-    return u < rule.share ? rule.share : u;
+EPTQ_HD long long share_of(long long all_blocks, int n_shares, CutRule& rule) {
+    const long long u = quotient(all_blocks + n_shares - 1, n_shares), size = u < rule.share ? rule.share : u;
+    if (size < 8 * rule.near) rule.near = static_cast<int>(size / 8);
+    return size;
 }
 
 // How far a cut at place p moves.

@@ -116,6 +116,18 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// The lane whose bit BIT is clear gives b and gets the other's a for it, the other the other way round.
+template <int BIT>
+__device__ __forceinline__ void swap_units(uint4& a, uint4& b, int lane) {
+    const bool upper = lane & BIT;
+    uint4 give = upper ? a : b;
+    give.x = __shfl_xor_sync(0xffffffffu, give.x, BIT);
+    give.y = __shfl_xor_sync(0xffffffffu, give.y, BIT);
+    give.z = __shfl_xor_sync(0xffffffffu, give.z, BIT);
+    give.w = __shfl_xor_sync(0xffffffffu, give.w, BIT);
+    if (upper) a = give; else b = give;
+}
+
 // An item and the blocks of keys that either half of its rows sees.
 struct HalvedItem {
     Item it;
@@ -175,7 +187,7 @@ struct Shared {
 template <typename T, int HD, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttentionArgs p, const CutRule rule) {
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttentionArgs p, CutRule rule) {
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Shared sh;
     constexpr int kBoxes = HD / 64;
@@ -233,7 +245,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     bool ok = true;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
             // ---------------- items, Q and K
             ShareWalk walk;
@@ -352,7 +364,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     warp_wait(smem_u32(&sh.v_full[i % kVSlots]), (i / kVSlots) & 1u, &never);
             }
         } else if (warp == 1) {
-            // ---------------- MMA
+            // ---------------- MMA.  The whole warp walks, one lane issues: what is the same for all lanes stays in uniform
+            // registers, as the instructions want it (one lane walking alone was 15 % slower).
             const uint32_t qk = instr_desc(kKeyBlock, kBf16, false, p.negative != 0);
             constexpr uint32_t pv = instr_desc(HD, kBf16, true, false);
             const uint64_t q_desc = desc_sw128(smem_u32(tiles), 16), k_desc = desc_sw128(smem_u32(k_tiles), 16);
@@ -380,14 +393,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                                 ok = warp_wait(smem_u32(&sh.v_full[v_slot]), (v_seq / kVSlots) & 1u, &sh.stop);
                                 if (!ok) break;
                                 v_here = true;
-                                if (live & 15) {                  // clear the rest of the last 16 keys
-                                    const int gone = 16 - (live & 15);
-                                    unsigned char* const v = v_tiles + v_slot * kTile + live * 128;
-                                    for (int i = lane; i < gone * 8 * kBoxes; i += 32)
-                                        *reinterpret_cast<uint4*>(v + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
-                                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                                    __syncwarp();
-                                }
                             }
                             if (j == 1) {                         // the last item's O has been read
                                 ok = warp_wait(smem_u32(&sh.o_empty[h]), (o_count[h] & 1u) ^ 1u, &sh.stop);
@@ -456,7 +461,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---------------- softmax: thread = row of half h
         const int h = (warp - 4) >> 2;
         const int row = (warp & 3) * 32 + lane;
@@ -488,6 +493,19 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int key0 = (it.block + j) * kKeyBlock;
                 const int allowed = seen + 1 - key0;
                 const unsigned lost = PAGED ? sh.lost[(block_seq + j) % kKeysSeen] : 0u;
+                const int rest = it.keys - key0;                               // keys that exist, from this block's first on
+                if (rest < kKeyBlock && (rest & 15) != 0) {
+                    // What lies behind the last key may be anything; its weight is zero, and zero times it must be too.  The
+                    // product ends with the last key's 16: clear the rest of those in V.
+                    const int slot = (block_seq + j) % kVSlots;
+                    ok = warp_wait(smem_u32(&sh.v_full[slot]), ((block_seq + j) / kVSlots) & 1u, &sh.stop);
+                    if (!ok) break;
+                    const int gone = rest > 0 ? 16 - (rest & 15) : 0;
+                    unsigned char* const v = v_tiles + slot * kTile + rest * 128;
+                    for (int i = row; i < gone * 8 * kBoxes; i += 128)
+                        *reinterpret_cast<uint4*>(v + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 if (__any_sync(0xffffffffu, allowed < kKeyBlock) || (PAGED && lost != 0)) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
@@ -553,25 +571,30 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             if (it.slot < 0) {
                 if (count > 0) {
-                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                    uint16_t* const dst = p.out + (static_cast<long long>(it.row + token) * p.n_heads + it.head + head) * HD;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    // A lane holds a row; rows are far apart in `out`, and a store that touches 32 of them takes the load/store unit 32
+                    // turns (4450 cycles a tile).  So four lanes exchange what they hold, 16 bytes at a time, and write 64
+                    // bytes of one row after the other together.
+                    const long long mine = live_row ? (static_cast<long long>(it.row + token) * p.n_heads + it.head + head) * HD : -1;
+                    long long at[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) at[r] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + r);
 #pragma unroll 1
                     for (int c = 0; c < HD / 32; ++c) {
                         float o[32];
                         tmem_ld32(o_at + c * 32, o);
                         tmem_wait_ld();
-                        if (!live_row) continue;
+                        uint4 u[4];
+                        unsigned* const w = reinterpret_cast<unsigned*>(u);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 v;
-                            unsigned* const w = reinterpret_cast<unsigned*>(&v);
+                        for (int i = 0; i < 16; ++i) w[i] = sum == 0.f ? 0u : Pair16<T>::pack(o[2 * i] * inv, o[2 * i + 1] * inv);
+                        swap_units<1>(u[0], u[1], lane);
+                        swap_units<1>(u[2], u[3], lane);
+                        swap_units<2>(u[0], u[2], lane);
+                        swap_units<2>(u[1], u[3], lane);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float a = o[i * 8 + 2 * e], b = o[i * 8 + 2 * e + 1];
-                                w[e] = sum == 0.f ? 0u : Pair16<T>::pack(a * inv, b * inv);
-                            }
-                            *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = v;
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            if (at[r] >= 0) *reinterpret_cast<uint4*>(p.out + at[r] + c * 32 + (lane & 3) * 8) = u[r];
                     }
                 }
             } else if (it.tokens > h * p.tokens_per_half) {
@@ -588,7 +611,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (!live_row) continue;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            reinterpret_cast<float4*>(piece + at_row * HD)[c * 8 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            reinterpret_cast<float4*>(piece)[(c * 8 + i) * 256 + at_row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
@@ -604,12 +627,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         sh.stop = 1;
         if (lane == 0 && p.status != nullptr) atomicExch(p.status, EPTQ_ERR_TIMEOUT);
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
-constexpr CutRule kRule = {8, 2, 1};
+constexpr CutRule kRule = {4, 2, 1};
 template <typename T, int HD, bool PAGED>
 int run(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {
     static std::once_flag once[64];

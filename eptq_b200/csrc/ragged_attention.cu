@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kJoinRows * HD / 8) attention_join_kernel(cons
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const CutTile c = p.cut_tiles[blockIdx.x];
     if (c.of == 0) return;
-    const int at_row = blockIdx.y * kJoinRows + threadIdx.x / (HD / 8), col = threadIdx.x % (HD / 8) * 8;
+    const int at_row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, col = threadIdx.x / kJoinRows * 8;
     const int half = at_row >> 7, row = at_row & 127;
     const int token = half * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
     if (row >= p.heads_per_tile * p.tokens_per_half || token >= c.tokens) return;
@@ -44,25 +44,37 @@ __global__ void __launch_bounds__(kJoinRows * HD / 8) attention_join_kernel(cons
     const float* const first = p.partial + (2 * blockIdx.x + 1) * size;
     const float* const others = p.partial + 2 * blockIdx.x * size;      // piece i at 2 i pieces behind, i = 1 ..
     const int stat = p.tile_rows * HD + at_row;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < c.of; ++i) {
-        const float* const piece = i == 0 ? first : others + 2 * i * size;
-        const float bias = __ldcg(piece + stat), sum = __ldcg(piece + stat + p.tile_rows);
-        if (sum != 0.f) top = fmaxf(top, bias);
-    }
-    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, all = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < c.of; ++i) {
-        const float* const piece = i == 0 ? first : others + 2 * i * size;
-        const float sum = __ldcg(piece + stat + p.tile_rows);
-        const float w = exp2_approx(__ldcg(piece + stat) - top);
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(piece + at_row * HD + col));
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(piece + at_row * HD + col) + 1);
-        if (sum == 0.f) continue;                                       // no key seen: its o was not written
-        all += sum * w;
-        o[0] += x.x * w; o[1] += x.y * w; o[2] += x.z * w; o[3] += x.w * w;
-        o[4] += y.x * w; o[5] += y.y * w; o[6] += y.z * w; o[7] += y.w * w;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, all = 0.f, top = -INFINITY;
+    constexpr int kAtOnce = 8;                                          // pieces whose reads are in flight together
+    for (int i0 = 0; i0 < c.of; i0 += kAtOnce) {
+        float bias[kAtOnce], sum[kAtOnce];
+        float4 x[kAtOnce], y[kAtOnce];
+        float high = top;
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+            const int i = min(i0 + n, c.of - 1);
+            const float* const piece = i == 0 ? first : others + 2 * i * size;
+            bias[n] = __ldcg(piece + stat);
+            sum[n] = i0 + n < c.of ? __ldcg(piece + stat + p.tile_rows) : 0.f;
+            x[n] = __ldcg(reinterpret_cast<const float4*>(piece) + col / 4 * p.tile_rows + at_row);
+            y[n] = __ldcg(reinterpret_cast<const float4*>(piece) + (col / 4 + 1) * p.tile_rows + at_row);
+        }
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n)
+            if (sum[n] != 0.f) high = fmaxf(high, bias[n]);
+        const float keep = top == -INFINITY ? 0.f : exp2_approx(top - high);
+        top = high;
+        all *= keep;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] *= keep;
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+            if (sum[n] == 0.f) continue;                                // no key seen: its o was not written
+            const float w = exp2_approx(bias[n] - top);
+            all += sum[n] * w;
+            o[0] += x[n].x * w; o[1] += x[n].y * w; o[2] += x[n].z * w; o[3] += x[n].w * w;
+            o[4] += y[n].x * w; o[5] += y[n].y * w; o[6] += y[n].z * w; o[7] += y[n].w * w;
+        }
     }
     const float inv = all == 0.f ? 0.f : 1.f / all;
     uint4 v;
