@@ -110,6 +110,7 @@ struct Share {
     long long begin, end;        // in blocks of keys
     long long size;              // of an uncut share
     int request;                 // that holds the begin
+    Request r;                   // its lengths
     Place at;                    // the begin there
 };
 template <int kThreads>
@@ -118,6 +119,7 @@ struct ShareScratch {
     long long before[2];         // blocks before the request that holds the share's begin and its end
     int request[2];
     long long cut[2];
+    Request r;
     Place at;
 };
 
@@ -200,12 +202,14 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, in
                 at.block += step;
                 if (at.block == at.blocks) { at.block = 0; ++at.tile; }
                 sh.at = at;
+                sh.r = r;
             }
         }
         if (lane == 0) sh.cut[warp] = cut;
     }
     __syncthreads();
     share.request = sh.request[0];
+    share.r = sh.r;
     share.at = sh.at;
     share.begin = sh.cut[0];
     share.end = sh.cut[1];
@@ -231,7 +235,7 @@ struct ShareWalk {
 
     __device__ __forceinline__ void start(const AttentionArgs& p, const Share& s) {
         b = s.request;
-        r = load_request(p, b);
+        r = s.r;
         now = s.at;
         left = s.end - s.begin;
         flat = s.begin;

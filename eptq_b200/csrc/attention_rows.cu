@@ -1,11 +1,12 @@
-// Causal attention of few rows over a paged cache, sm_100a: the single token of every running request, or a handful.
+// Causal attention of few rows over a paged cache, sm_100a: the single token of every running request, or a few of them.
 //
-// Every key and value is read once and meets at most 32 rows, so the kernel is bound by how fast the cache can be read;
-// the products run on mma.sync (16 rows x 8 keys x 16), whose rate is far above what the reads can feed.  What counts is
-// bytes in flight: each of a block's four warps works alone, on its own 16 keys (32 of head 64) of every block of keys,
-// with its own ring of TMA stages (4 KB of keys and 4 KB of values each) that its own lanes refill; no warp waits for
-// another before the end of a row tile, where the four results meet in shared memory.  Three blocks an SM (two with 32
-// rows) cover each other's ends and starts.  Which keys a block takes: attention_schedule.cuh.
+// Every key and value is read once and meets at most 16 rows (the query heads of one key/value head times the request's
+// tokens), so the kernel is bound by how fast the cache can be read; the products run on mma.sync (16 rows x 8 keys x 16),
+// whose rate is far above what the reads can feed.  What counts is bytes in flight: each of a block's four warps works alone,
+// on its own 16 keys (32 of head 64) of every block of keys, with its own ring of TMA stages (4 KB of keys and 4 KB of values
+// each) that its own lanes refill; no warp waits for another before the end of a row tile, where the four results meet in
+// shared memory.  Three blocks an SM cover each other's ends and starts (refilling on into the next tile, with shared memory
+// of its own for the results, was 5 to 8 % slower).  Which keys a block takes: attention_schedule.cuh.
 
 #include <mutex>
 
@@ -18,13 +19,15 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
+constexpr int kRows = 16;
+constexpr int kBlocksPerSm = 3;
+constexpr int kStages = 2;
 constexpr int kStageBytes = 8192;
 constexpr int kBoxBytes = 16 * 128;                       // 16 keys x 64 columns
+constexpr int kPad = 8;                                   // floats behind a row of results: rows begin in different banks
 __host__ __device__ constexpr int unit_keys(int hd) { return 2048 / hd; }
 __host__ __device__ constexpr int key_block(int hd) { return kWarps * unit_keys(hd); }
-__host__ __device__ constexpr int blocks_per_sm(int mt) { return mt == 1 ? 3 : 2; }
-__host__ __device__ constexpr int stages(int mt) { return mt == 1 ? 2 : 3; }
-__host__ __device__ constexpr int smem_bytes(int mt) { return kWarps * stages(mt) * kStageBytes + 1024; }
+constexpr int kSmemBytes = kWarps * kStages * kStageBytes + 1024;
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -50,20 +53,19 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// MT: 16-row tiles.
-template <typename T, int HD, int MT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(MT))
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ AttentionArgs p, CutRule rule) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ __align__(8) unsigned long long full[kWarps][stages(MT)];
+    __shared__ __align__(8) unsigned long long full[kWarps][kStages];
     __shared__ ShareScratch<kThreads> share_scratch;
-    __shared__ float2 stats[kWarps][16 * MT];              // reference and sum of a warp's rows
+    __shared__ float2 stats[kWarps][kRows];                // reference and sum of a warp's rows
     __shared__ int stop;
-    constexpr int kStages = stages(MT), kUnit = unit_keys(HD), kBlock = key_block(HD);
+    constexpr int kUnit = unit_keys(HD), kBlock = key_block(HD);
     constexpr int kSub = kUnit / 16, kCols = HD / 64;      // boxes of 16 keys, of 64 columns: two in all for keys, two for values
-    constexpr int kPitch = HD + 8;                         // floats from row to row of a warp's o in shared memory
-    static_assert(kSub * kCols == 2 && 16 * MT * kPitch * 4 <= kStages * kStageBytes, "stage layout");
+    constexpr int kPitch = HD + kPad;
+    static_assert(kSub * kCols == 2 && kRows * kPitch * 4 <= kStages * kStageBytes, "stage layout");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     unsigned char* const ring = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u) + warp * (kStages * kStageBytes);
     const unsigned ring_at = smem_u32(ring);
@@ -99,7 +101,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int units = max(0, min(it.blocks, ((it.keys + kUnit - 1) / kUnit - unit0 + kWarps - 1) / kWarps));
         const int kv_head = it.head / p.kv_group;
         const int* const table = p.tables + it.request * p.table_stride;
-        // lanes 0-3 each load one box of a unit: key or value, and which of the two
+        // lanes 0-3 each load one box of a unit: of keys or values, and which of the two
         const int sub = kSub == 2 ? lane & 1 : 0, col64 = kSub == 2 ? 0 : lane & 1;
         auto page_of = [&](int i) {                        // page of this lane's box of unit i
             const int key = (unit0 + i * kWarps) * kUnit + sub * 16;
@@ -129,30 +131,25 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         int next_page = page[kStages];
 
         // q as the product's left operand, and what each of this thread's rows sees
-        unsigned q[MT][HD / 16][4];
-        int seen[MT][2];
+        unsigned q[HD / 16][4];
+        int seen[2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int e = 0; e < 2; ++e) {
+            const int row = e * 8 + g, token = row / p.heads_per_tile;
+            const bool live = row < p.heads_per_tile * tile_tokens && token < it.tokens;
+            seen[e] = it.seen + min(token, it.tokens - 1);
+            const uint16_t* const src = p.q + (it.row + token) * p.q_stride + (it.head + row % p.heads_per_tile) * HD + 2 * t;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = m * 16 + e * 8 + g, token = row / p.heads_per_tile;
-                const bool live = row < p.heads_per_tile * tile_tokens && token < it.tokens;
-                seen[m][e] = it.seen + min(token, it.tokens - 1);
-                const uint16_t* const src = p.q + (it.row + token) * p.q_stride + (it.head + row % p.heads_per_tile) * HD + 2 * t;
+            for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        q[m][k][2 * c + e] = live ? __ldg(reinterpret_cast<const unsigned*>(src + k * 16 + c * 8)) : 0u;
-            }
-        float o[MT][HD / 8][4], top[MT][2], bias[MT][2], sum[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) { top[m][e] = -INFINITY; bias[m][e] = 0.f; sum[m][e] = 0.f; }
+                for (int c = 0; c < 2; ++c)
+                    q[k][2 * c + e] = live ? __ldg(reinterpret_cast<const unsigned*>(src + k * 16 + c * 8)) : 0u;
         }
+        float o[HD / 8][4], top[2], bias[2], sum[2];
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { top[e] = -INFINITY; bias[e] = 0.f; sum[e] = 0.f; }
 
         for (int i = 0; i < units; ++i) {
             const int s = used % kStages;
@@ -161,82 +158,67 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             ++used;
             const unsigned k_at = ring_at + s * kStageBytes, v_at = k_at + kStageBytes / 2;
             const int key0 = (unit0 + i * kWarps) * kUnit;
-            float z[MT][2 * kSub][4];
+            const unsigned gone = (lost >> (2 * s)) & 3u;
+            float z[2 * kSub][4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < 2 * kSub; ++n) z[n][0] = z[n][1] = z[n][2] = z[n][3] = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2 * kSub; ++n) z[m][n][0] = z[m][n][1] = z[m][n][2] = z[m][n][3] = 0.f;
+            for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
-            for (int b = 0; b < kSub; ++b)
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
+                for (int b = 0; b < kSub; ++b) {
                     unsigned r[4];
                     const int key = (lane >> 4) * 8 + (lane & 7), chunk = (k & 3) * 2 + ((lane >> 3) & 1);
                     ldmatrix4(r, k_at + (b * kCols + (k >> 2)) * kBoxBytes + key * 128 + ((chunk ^ (key & 7)) << 4));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        mma<T>(z[m][2 * b], q[m][k], r[0], r[1]);
-                        mma<T>(z[m][2 * b + 1], q[m][k], r[2], r[3]);
-                    }
+                    mma<T>(z[2 * b], q[k], r[0], r[1]);
+                    mma<T>(z[2 * b + 1], q[k], r[2], r[3]);
                 }
-            const unsigned gone = (lost >> (2 * s)) & 3u;
             if (p.negative) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int n = 0; n < 2 * kSub; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) z[m][n][c] = -z[m][n][c];
-            }
-            if (it.seen + 1 - key0 < kUnit || gone != 0) {     // the first token sees the fewest keys
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int n = 0; n < 2 * kSub; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (key0 + n * 8 + 2 * t + (c & 1) > seen[m][c >> 1] || ((gone >> (n >> 1)) & 1u)) z[m][n][c] = -INFINITY;
-            }
-            float high[MT][2];
-            bool any = false;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v = z[m][0][2 * e];
-#pragma unroll
-                    for (int n = 0; n < 2 * kSub; ++n) v = fmaxf(v, fmaxf(z[m][n][2 * e], z[m][n][2 * e + 1]));
-                    high[m][e] = fmaxf(quad_max(v), top[m][e]);
-                    any |= top[m][e] == -INFINITY ? high[m][e] > -INFINITY : (high[m][e] - top[m][e]) * p.scale_log2 > kRescaleAt;
-                }
-            if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const bool first = top[m][e] == -INFINITY;
-                        const bool moves = first ? high[m][e] > -INFINITY : (high[m][e] - top[m][e]) * p.scale_log2 > kRescaleAt;
-                        const float new_bias = moves ? high[m][e] * p.scale_log2 - kExpOffset : bias[m][e];
-                        const float keep = first ? 1.f : exp2_approx(bias[m][e] - new_bias);
-                        top[m][e] = moves ? high[m][e] : top[m][e];
-                        bias[m][e] = new_bias;
-                        sum[m][e] *= keep;
-#pragma unroll
-                        for (int n = 0; n < HD / 8; ++n) { o[m][n][2 * e] *= keep; o[m][n][2 * e + 1] *= keep; }
-                    }
-            }
-            unsigned w[MT][kSub][4];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < 2 * kSub; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = exp2_approx(fmaf(z[m][n][2 * e], p.scale_log2, -bias[m][e]));
-                        const float b = exp2_approx(fmaf(z[m][n][2 * e + 1], p.scale_log2, -bias[m][e]));
-                        sum[m][e] += a + b;
-                        w[m][n >> 1][(n & 1) * 2 + e] = Pair16<T>::pack(a, b);
-                    }
+                    for (int c = 0; c < 4; ++c) z[n][c] = -z[n][c];
+            }
+            if (it.seen + 1 - key0 < kUnit || gone != 0) {     // the first token sees the fewest keys
+#pragma unroll
+                for (int n = 0; n < 2 * kSub; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (key0 + n * 8 + 2 * t + (c & 1) > seen[c >> 1] || ((gone >> (n >> 1)) & 1u)) z[n][c] = -INFINITY;
+            }
+            float high[2];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float v = z[0][2 * e];
+#pragma unroll
+                for (int n = 0; n < 2 * kSub; ++n) v = fmaxf(v, fmaxf(z[n][2 * e], z[n][2 * e + 1]));
+                high[e] = fmaxf(quad_max(v), top[e]);
+                any |= top[e] == -INFINITY ? high[e] > -INFINITY : (high[e] - top[e]) * p.scale_log2 > kRescaleAt;
+            }
+            if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const bool none = top[e] == -INFINITY;
+                    const bool moves = none ? high[e] > -INFINITY : (high[e] - top[e]) * p.scale_log2 > kRescaleAt;
+                    const float new_bias = moves ? high[e] * p.scale_log2 - kExpOffset : bias[e];
+                    const float keep = none ? 1.f : exp2_approx(bias[e] - new_bias);
+                    top[e] = moves ? high[e] : top[e];
+                    bias[e] = new_bias;
+                    sum[e] *= keep;
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) { o[n][2 * e] *= keep; o[n][2 * e + 1] *= keep; }
+                }
+            }
+            unsigned w[kSub][4];
+#pragma unroll
+            for (int n = 0; n < 2 * kSub; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float a = exp2_approx(fmaf(z[n][2 * e], p.scale_log2, -bias[e]));
+                    const float b = exp2_approx(fmaf(z[n][2 * e + 1], p.scale_log2, -bias[e]));
+                    sum[e] += a + b;
+                    w[n >> 1][(n & 1) * 2 + e] = Pair16<T>::pack(a, b);
+                }
             const bool tail = it.keys - key0 < kUnit;           // values behind the last key may be anything: clear them
 #pragma unroll
             for (int b = 0; b < kSub; ++b) {
@@ -252,11 +234,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const int key = ((lane >> 3) & 1) * 8 + (lane & 7), chunk = (n & 3) * 2 + (lane >> 4);
                     ldmatrix4_trans(r, v_at + (b * kCols + (n >> 2)) * kBoxBytes + key * 128 + ((chunk ^ (key & 7)) << 4));
                     if (tail) { r[0] &= keep0; r[1] &= keep1; r[2] &= keep0; r[3] &= keep1; }
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        mma<T>(o[m][2 * n], w[m][b], r[0], r[1]);
-                        mma<T>(o[m][2 * n + 1], w[m][b], r[2], r[3]);
-                    }
+                    mma<T>(o[2 * n], w[b], r[0], r[1]);
+                    mma<T>(o[2 * n + 1], w[b], r[2], r[3]);
                 }
             }
             __syncwarp();                                       // all lanes have read the stage
@@ -268,19 +247,17 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
 
         // the four warps' results meet; each lies where its stages were
-        float* const mine = reinterpret_cast<float*>(ring);
         if (ok) {
+            float* const mine = reinterpret_cast<float*>(ring);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int e = 0; e < 2; ++e) {
+                const int row = e * 8 + g;
+                const float all = quad_sum(sum[e]);
+                if (t == 0) stats[warp][row] = make_float2(bias[e], all);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = m * 16 + e * 8 + g;
-                    const float all = quad_sum(sum[m][e]);
-                    if (t == 0) stats[warp][row] = make_float2(bias[m][e], all);
-#pragma unroll
-                    for (int n = 0; n < HD / 8; ++n)
-                        *reinterpret_cast<float2*>(mine + row * kPitch + n * 8 + 2 * t) = make_float2(o[m][n][2 * e], o[m][n][2 * e + 1]);
-                }
+                for (int n = 0; n < HD / 8; ++n)
+                    *reinterpret_cast<float2*>(mine + row * kPitch + n * 8 + 2 * t) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+            }
         } else {
             stop = 1;
         }
@@ -288,9 +265,9 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         ok = *static_cast<volatile int*>(&stop) == 0;
         if (!ok) break;
         const float* const rings = reinterpret_cast<const float*>(ring - warp * (kStages * kStageBytes));
-        for (int x = tid; x < 16 * MT * (HD / 8); x += kThreads) {
-            const int row = x / (HD / 8), col = x % (HD / 8) * 8, token = row / p.heads_per_tile;
-            if (row >= p.heads_per_tile * tile_tokens || token >= it.tokens) continue;
+        const int rows = p.heads_per_tile * min(it.tokens, tile_tokens);
+        for (int x = tid; x < rows * (HD / 4); x += kThreads) {
+            const int row = x / (HD / 4), col = x % (HD / 4) * 4;
             float2 st[kWarps];
             float high = -INFINITY;
 #pragma unroll
@@ -298,31 +275,27 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 st[w] = stats[w][row];
                 if (st[w].y != 0.f) high = fmaxf(high, st[w].x);
             }
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, all = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float all = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 if (st[w].y == 0.f) continue;
                 const float f = exp2_approx(st[w].x - high);
-                const float* const src = rings + w * (kStages * kStageBytes / 4) + row * kPitch + col;
+                const float4 y = *reinterpret_cast<const float4*>(rings + w * (kStages * kStageBytes / 4) + row * kPitch + col);
                 all += st[w].y * f;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) v[c] += src[c] * f;
+                v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
             }
             if (it.slot < 0) {
                 const float inv = all == 0.f ? 0.f : 1.f / all;
-                uint4 out;
-                out.x = Pair16<T>::pack(v[0] * inv, v[1] * inv);
-                out.y = Pair16<T>::pack(v[2] * inv, v[3] * inv);
-                out.z = Pair16<T>::pack(v[4] * inv, v[5] * inv);
-                out.w = Pair16<T>::pack(v[6] * inv, v[7] * inv);
-                *reinterpret_cast<uint4*>(p.out + (static_cast<long long>(it.row + token) * p.n_heads + it.head + row % p.heads_per_tile) * HD + col) = out;
+                const int token = row / p.heads_per_tile;
+                *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(it.row + token) * p.n_heads + it.head + row % p.heads_per_tile) * HD + col) =
+                    make_uint2(Pair16<T>::pack(v.x * inv, v.y * inv), Pair16<T>::pack(v.z * inv, v.w * inv));
             } else {
-                float* const piece = p.partial + it.slot * piece_floats(16 * MT, HD);
-                reinterpret_cast<float4*>(piece)[col / 4 * (16 * MT) + row] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(piece)[(col / 4 + 1) * (16 * MT) + row] = make_float4(v[4], v[5], v[6], v[7]);
+                float* const piece = p.partial + it.slot * piece_floats(kRows, HD);
+                reinterpret_cast<float4*>(piece)[col / 4 * kRows + row] = v;
                 if (col == 0) {
-                    piece[16 * MT * HD + row] = all == 0.f ? 0.f : high;
-                    piece[16 * MT * HD + 16 * MT + row] = all;
+                    piece[kRows * HD + row] = all == 0.f ? 0.f : high;
+                    piece[kRows * HD + kRows + row] = all;
                 }
             }
         }
@@ -338,44 +311,36 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
 }
 
-constexpr CutRule kRule = {4, 1, 2};
+constexpr CutRule kRule = {2, 1, 1};
 
-template <typename T, int HD, int MT>
+template <typename T, int HD>
 int run(const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {
     static std::once_flag once[64];
     static bool set[64] = {};
     std::call_once(once[dev], [dev]() {
-        set[dev] = cudaFuncSetAttribute(attention_rows_kernel<T, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MT)) == cudaSuccess;
+        set[dev] = cudaFuncSetAttribute(attention_rows_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
     });
     if (!set[dev]) return EPTQ_ERR_LAUNCH;
-    return launch_dependent(attention_rows_kernel<T, HD, MT>, dim3(kSms * blocks_per_sm(MT)), kThreads, smem_bytes(MT), stream, k, v, args, kRule);
+    return launch_dependent(attention_rows_kernel<T, HD>, dim3(kSms * kBlocksPerSm), kThreads, kSmemBytes, stream, k, v, args, kRule);
 }
-
-int row_tiles(const EptqAttention& a) { return static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > 16 ? 2 : 1; }
 
 }  // namespace
 
 AttentionPlan attention_rows_plan(const EptqAttention& a) {
-    const int mt = row_tiles(a);
     AttentionPlan plan;
-    plan.shares = kSms * blocks_per_sm(mt);
-    plan.tile_rows = 16 * mt;
+    plan.shares = kSms * kBlocksPerSm;
+    plan.tile_rows = kRows;
     plan.may_cut = static_cast<long long>(a.table_width) * a.page_size > static_cast<long long>(kRule.least) * key_block(a.head_dim);
     return plan;
 }
 
 int launch_attention_rows(const EptqAttention& a, AttentionArgs& p, int dev, cudaStream_t stream) {
-    const int mt = row_tiles(a);
-    p.heads_per_tile = heads_in(p.kv_group, 16 * mt);
-    p.tokens_per_half = 16 * mt / p.heads_per_tile;
+    p.heads_per_tile = heads_in(p.kv_group, kRows);
+    p.tokens_per_half = kRows / p.heads_per_tile;
     CUtensorMap k, v;
     if (!encode_page_maps(&k, &v, a, 16)) return EPTQ_ERR_LAUNCH;
-    if (a.dtype == EPTQ_FP16) {
-        if (a.head_dim == 128) return mt == 1 ? run<__half, 128, 1>(k, v, p, dev, stream) : run<__half, 128, 2>(k, v, p, dev, stream);
-        return mt == 1 ? run<__half, 64, 1>(k, v, p, dev, stream) : run<__half, 64, 2>(k, v, p, dev, stream);
-    }
-    if (a.head_dim == 128) return mt == 1 ? run<__nv_bfloat16, 128, 1>(k, v, p, dev, stream) : run<__nv_bfloat16, 128, 2>(k, v, p, dev, stream);
-    return mt == 1 ? run<__nv_bfloat16, 64, 1>(k, v, p, dev, stream) : run<__nv_bfloat16, 64, 2>(k, v, p, dev, stream);
+    if (a.dtype == EPTQ_FP16) return a.head_dim == 128 ? run<__half, 128>(k, v, p, dev, stream) : run<__half, 64>(k, v, p, dev, stream);
+    return a.head_dim == 128 ? run<__nv_bfloat16, 128>(k, v, p, dev, stream) : run<__nv_bfloat16, 64>(k, v, p, dev, stream);
 }
 
 }  // namespace eptq

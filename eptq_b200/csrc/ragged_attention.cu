@@ -27,35 +27,42 @@ PFN_cuTensorMapEncodeTiled_v12000 attention_map_encoder() {
 
 namespace {
 
-// Block (share, 16 rows of its cut tile), 8 columns of one row per thread.  Pieces are added in the order of the keys.
-constexpr int kJoinRows = 16;
+// Block (share, 16 rows of its cut tile), 8 columns of one row per thread.  Where the tile has 8 rows or 4 -- a long request of one
+// token has 50 pieces of 4 rows -- two or four sets of threads take every second or fourth piece.  Pieces are added in an order
+// that depends on the tile and its cuts alone.
+constexpr int kJoinRows = 16, kMostSets = 4;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinRows * HD / 8) attention_join_kernel(const __grid_constant__ AttentionArgs p) {
+    constexpr int kCols = HD / 8;
+    __shared__ float parts[10][kJoinRows * kCols];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const CutTile c = p.cut_tiles[blockIdx.x];
     if (c.of == 0) return;
-    const int at_row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, col = threadIdx.x / kJoinRows * 8;
+    const int tile_rows = p.tile_rows < 256 ? min(c.tokens, p.tokens_per_half) * p.heads_per_tile : kJoinRows;
+    const int sets = tile_rows <= kJoinRows / 4 ? 4 : tile_rows <= kJoinRows / 2 ? 2 : 1, set_rows = kJoinRows / sets;
+    const int in_block = threadIdx.x % kJoinRows, set = in_block / set_rows;
+    const int at_row = blockIdx.y * kJoinRows + in_block % set_rows, col = threadIdx.x / kJoinRows * 8;
     const int half = at_row >> 7, row = at_row & 127;
     const int token = half * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
-    if (row >= p.heads_per_tile * p.tokens_per_half || token >= c.tokens) return;
+    const bool live = row < p.heads_per_tile * p.tokens_per_half && token < c.tokens;
     const long long size = piece_floats(p.tile_rows, HD);
     const float* const first = p.partial + (2 * blockIdx.x + 1) * size;
     const float* const others = p.partial + 2 * blockIdx.x * size;      // piece i at 2 i pieces behind, i = 1 ..
     const int stat = p.tile_rows * HD + at_row;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, all = 0.f, top = -INFINITY;
     constexpr int kAtOnce = 8;                                          // pieces whose reads are in flight together
-    for (int i0 = 0; i0 < c.of; i0 += kAtOnce) {
+    for (int i0 = set; live && i0 < c.of; i0 += kAtOnce * sets) {
         float bias[kAtOnce], sum[kAtOnce];
         float4 x[kAtOnce], y[kAtOnce];
         float high = top;
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-            const int i = min(i0 + n, c.of - 1);
+            const int i = min(i0 + n * sets, c.of - 1);
             const float* const piece = i == 0 ? first : others + 2 * i * size;
             bias[n] = __ldcg(piece + stat);
-            sum[n] = i0 + n < c.of ? __ldcg(piece + stat + p.tile_rows) : 0.f;
+            sum[n] = i0 + n * sets < c.of ? __ldcg(piece + stat + p.tile_rows) : 0.f;
             x[n] = __ldcg(reinterpret_cast<const float4*>(piece) + col / 4 * p.tile_rows + at_row);
             y[n] = __ldcg(reinterpret_cast<const float4*>(piece) + (col / 4 + 1) * p.tile_rows + at_row);
         }
@@ -76,6 +83,26 @@ __global__ void __launch_bounds__(kJoinRows * HD / 8) attention_join_kernel(cons
             o[4] += y[n].x * w; o[5] += y[n].y * w; o[6] += y[n].z * w; o[7] += y[n].w * w;
         }
     }
+    if (sets > 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) parts[e][threadIdx.x] = o[e];
+        parts[8][threadIdx.x] = all;
+        parts[9][threadIdx.x] = top;
+        __syncthreads();
+        if (set > 0 || !live) return;
+        for (int s = 1; s < sets; ++s) {
+            const int other = threadIdx.x + s * set_rows;
+            const float sum = parts[8][other];
+            if (sum == 0.f) continue;
+            const float high = fmaxf(top, parts[9][other]);
+            const float keep = all == 0.f ? 0.f : exp2_approx(top - high), w = exp2_approx(parts[9][other] - high);
+            top = high;
+            all = all * keep + sum * w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = o[e] * keep + parts[e][other] * w;
+        }
+    }
+    if (!live) return;
     const float inv = all == 0.f ? 0.f : 1.f / all;
     uint4 v;
     v.x = Pair16<T>::pack(o[0] * inv, o[1] * inv);
@@ -113,8 +140,11 @@ int check(const EptqAttention& a) {
     return EPTQ_OK;
 }
 
-// Rows of one key/value head of a request from which the tensor-core kernel takes a paged call.
-constexpr int kTensorRows = 32;
+// Up to 16 rows of one key/value head of a request fill the smallest matrix tile and the call is bound by the cache's reads;
+// above, the tcgen05 kernel reads as fast and multiplies faster: 32 rows over 4000 keys, 8 requests with 8 key/value heads,
+// 40 against 49 us (as two 16-row tiles), 64 rows over 1000 keys, 4 requests, 16 against 19 us; the other way round where heads
+// of 64 are many and short (20 rows over 1000 keys, 16 requests of 12 heads: 34 against 22 us).
+constexpr int kTensorRows = 16;
 
 bool on_tensor_cores(const EptqAttention& a) {
     return a.page_size == 0 || static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > kTensorRows;
