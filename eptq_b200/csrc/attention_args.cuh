@@ -107,7 +107,7 @@ __device__ __forceinline__ Request load_request(const AttentionArgs& p, int b) {
 
 // The part of the work that falls to one block of the launch.
 struct Share {
-    long long begin, end;        // in blocks of keys
+    long long begin, end;        // in what the sequence counts
     long long size;              // of an uncut share
     int request;                 // that holds the begin
     Request r;                   // its lengths
@@ -140,7 +140,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, in
                 w[i] = 0;
                 if (b < p.batch) {
                     const Request r = load_request(p, b);
-                    w[i] = blocks_before(r, tile, kb, tiles_of(r, tile)) * groups;
+                    w[i] = cost_before(r, tile, kb, rule, tiles_of(r, tile)) * groups;
                 }
                 mine += w[i];
             }
@@ -186,21 +186,18 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& p, int tile, in
         if (end < all) {
             const Request r = load_request(p, sh.request[warp]);
             // 32 tiles looked at in each round: the sums before a tile take a few divisions
-            Place at = place_of(r, tile, kb, end - sh.before[warp], [&](int lo, int hi, long long y) {
+            Place at = place_of(r, tile, kb, rule, end - sh.before[warp], [&](int lo, int hi, long long y) {
                 while (lo < hi) {
                     const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
-                    const bool begins = i <= hi && blocks_before(r, tile, kb, i) <= y;
+                    const bool begins = i <= hi && cost_before(r, tile, kb, rule, i) <= y;
                     const int n = __popc(__ballot_sync(0xffffffffu, begins));      // beginnings rise: the first n lanes
                     lo += n * step;
                     hi = min(hi, lo + step - 1);
                 }
                 return lo;
             });
-            const int step = moved(at, rule);
-            cut = end + step;
+            cut = moved(at, rule, end);
             if (warp == 0 && lane == 0) {
-                at.block += step;
-                if (at.block == at.blocks) { at.block = 0; ++at.tile; }
                 sh.at = at;
                 sh.r = r;
             }
@@ -259,12 +256,13 @@ struct ShareWalk {
         it.seen = r.past + now.tile * tile;
         it.keys = max(0, it.seen + it.tokens);
         it.block = now.block;
-        it.blocks = static_cast<int>(min(static_cast<long long>(blocks - now.block), left));
+        const int ahead = now.block == 0 ? rule.tile : 0;
+        it.blocks = static_cast<int>(min(static_cast<long long>(blocks - now.block), left - ahead));
         const bool whole = it.blocks == blocks;
         it.slot = whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (it.block == 0 ? 1 : 0);
-        it.of = whole || it.block != 0 ? 0 : last_share(flat + blocks, size, rule) - static_cast<int>(blockIdx.x) + 1;
-        left -= it.blocks;
-        flat += it.blocks;
+        it.of = whole || it.block != 0 ? 0 : last_share(flat + ahead + blocks, size, rule) - static_cast<int>(blockIdx.x) + 1;
+        left -= ahead + it.blocks;
+        flat += ahead + it.blocks;
         now.block = 0;
         ++now.tile;
         return true;

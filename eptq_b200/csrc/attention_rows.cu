@@ -311,7 +311,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
 }
 
-constexpr CutRule kRule = {2, 1, 1};
+constexpr CutRule kRule = {2, 1, 1, 1};
 
 template <typename T, int HD>
 int run(const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {

@@ -6,6 +6,7 @@
 // sequence -- request, head group, row tile, block -- and launch block c takes the blocks from cut(c) to cut(c + 1).  Cuts
 // at equal distances balance requests of any lengths without knowing them on the host; a tile cut in two or more is joined
 // from partial results.  Joining costs about as much as a few blocks, so a cut moves to the end of a tile that is short or near.
+// Beginning and ending a tile costs time too: each counts as rule.tile blocks more, ahead of its first one.
 #pragma once
 
 #include <stdint.h>
@@ -22,6 +23,7 @@ struct CutRule {
     int least;     // a tile of at most this many blocks is not cut
     int near;      // a cut this near an end of its tile moves there, where that is at most an eighth of a share
     int share;     // least blocks of a share
+    int tile;      // blocks that a tile's beginning and end count as
 };
 
 struct Request {
@@ -120,23 +122,31 @@ EPTQ_HD long long blocks_before(const Request& r, int tile, int kb, int i) {
     return sum;
 }
 
+// What the row tiles before tile i count.
+EPTQ_HD long long cost_before(const Request& r, int tile, int kb, const CutRule& rule, int i) {
+    return blocks_before(r, tile, kb, i) + static_cast<long long>(i) * rule.tile;
+}
+
 // A place in the sequence inside one request.
 struct Place {
     int group, tile, block;    // head group, row tile, block of keys
     int blocks;                // of that row tile
+    int ahead;                 // what the place counts ahead of the tile's first block (then block is 0)
 };
 
-// x = blocks of the request before the place, 0 <= x < groups * blocks_before(all tiles).  `last_tile_at(lo, hi, y)` gives the
+// x = what the request counts before the place, 0 <= x < groups * cost_before(all tiles).  `last_tile_at(lo, hi, y)` gives the
 // last tile of lo .. hi that begins at or before y.
 template <typename Search>
-EPTQ_HD Place place_of(const Request& r, int tile, int kb, long long x, const Search& last_tile_at) {
+EPTQ_HD Place place_of(const Request& r, int tile, int kb, const CutRule& rule, long long x, const Search& last_tile_at) {
     const int tiles = tiles_of(r, tile);
-    const long long per_group = blocks_before(r, tile, kb, tiles);
+    const long long per_group = cost_before(r, tile, kb, rule, tiles);
     Place p;
     p.group = static_cast<int>(quotient(x, per_group));
     const long long y = x - p.group * per_group;
     p.tile = last_tile_at(0, tiles - 1, y);
-    p.block = static_cast<int>(y - blocks_before(r, tile, kb, p.tile));
+    const int u = static_cast<int>(y - cost_before(r, tile, kb, rule, p.tile));
+    p.block = u > rule.tile ? u - rule.tile : 0;
+    p.ahead = u < rule.tile ? rule.tile - u : 0;
     p.blocks = blocks_of(r, tile, kb, p.tile);
     return p;
 }
@@ -147,13 +157,20 @@ EPTQ_HD long long share_of(long long all_blocks, int n_shares, CutRule& rule) {
     return size;
 }
 
-// How far a cut at place p moves.
-EPTQ_HD int moved(const Place& p, const CutRule& rule) {
-    if (p.block == 0) return 0;
-    if (p.blocks <= rule.least) return 2 * p.block < p.blocks ? -p.block : p.blocks - p.block;
-    if (p.block <= rule.near) return -p.block;
-    if (p.blocks - p.block <= rule.near) return p.blocks - p.block;
-    return 0;
+// How far a cut at place p moves, from there: to the tile's own begin, to its end, or not.  Returns what the place counts then.
+EPTQ_HD long long moved(Place& p, const CutRule& rule, long long x) {
+    if (p.block == 0) {                                                           // to the tile's begin
+        x -= rule.tile - p.ahead;
+    } else if (p.blocks <= rule.least ? 2 * p.block < p.blocks : p.block <= rule.near) {
+        x -= p.block + rule.tile;
+        p.block = 0;
+    } else if (p.blocks <= rule.least || p.blocks - p.block <= rule.near) {
+        x += p.blocks - p.block;
+        p.block = 0;
+        ++p.tile;
+    }
+    p.ahead = rule.tile;
+    return x;
 }
 
 // The last share that holds blocks of a cut tile which ends at `tile_end` in the sequence.
