@@ -53,6 +53,43 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
+// o += w v over the unit's keys, with `limit` set over its first `keys` keys; with SOME only for the rows that are named (of g
+// and of g + 8).
+template <typename T, int HD, bool SOME>
+__device__ __forceinline__ void product(float (&o)[HD / 8][4], const unsigned (&w)[unit_keys(HD) / 16][4], unsigned v_at, bool limit, int keys, bool lower, bool upper) {
+    constexpr int kSub = unit_keys(HD) / 16, kCols = HD / 64;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+    for (int b = 0; b < kSub; ++b) {
+        unsigned keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (limit) {
+            const int live = keys - b * 16 - 2 * t;
+            keep0 = live >= 2 ? 0xffffffffu : live == 1 ? 0xffffu : 0u;
+            keep1 = live >= 10 ? 0xffffffffu : live == 9 ? 0xffffu : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+            unsigned r[4];
+            const int key = ((lane >> 3) & 1) * 8 + (lane & 7), chunk = (n & 3) * 2 + (lane >> 4);
+            ldmatrix4_trans(r, v_at + (b * kCols + (n >> 2)) * kBoxBytes + key * 128 + ((chunk ^ (key & 7)) << 4));
+            if (limit) { r[0] &= keep0; r[1] &= keep1; r[2] &= keep0; r[3] &= keep1; }
+            if (SOME) {
+                float x[4], y[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { x[c] = o[2 * n][c]; y[c] = o[2 * n + 1][c]; }
+                mma<T>(x, w[b], r[0], r[1]);
+                mma<T>(y, w[b], r[2], r[3]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < 2 ? lower : upper) { o[2 * n][c] = x[c]; o[2 * n + 1][c] = y[c]; }
+            } else {
+                mma<T>(o[2 * n], w[b], r[0], r[1]);
+                mma<T>(o[2 * n + 1], w[b], r[2], r[3]);
+            }
+        }
+    }
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -219,24 +256,32 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     sum[e] += a + b;
                     w[n >> 1][(n & 1) * 2 + e] = Pair16<T>::pack(a, b);
                 }
-            const bool tail = it.keys - key0 < kUnit;           // values behind the last key may be anything: clear them
+            // Values behind the last key a row sees may be anything, and a weight of zero must make them zero: what lies
+            // behind the last token's is cleared.  Where the tokens see different keys of this unit and a value is not finite,
+            // every token's rows take their own product.
+            const bool tail = it.keys - key0 < kUnit;
+            bool apart = false;
+            if (it.tokens > 1 && it.seen + 1 - key0 < kUnit) {
+                unsigned acc = 0;                              // two zeros, or NaN where something was not finite
 #pragma unroll
-            for (int b = 0; b < kSub; ++b) {
-                unsigned keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                if (tail) {
-                    const int live = it.keys - key0 - b * 16 - 2 * t;
-                    keep0 = live >= 2 ? 0xffffffffu : live == 1 ? 0xffffu : 0u;
-                    keep1 = live >= 10 ? 0xffffffffu : live == 9 ? 0xffffu : 0u;
+                for (int i = 0; i < kStageBytes / 2 / 512; ++i) {
+                    const int at = i * 32 + lane, key = (at >> 7) % kSub * 16 + (at >> 3) % 16;        // 16-byte unit, its key
+                    const uint4 u = *reinterpret_cast<const uint4*>(ring + s * kStageBytes + kStageBytes / 2 + at * 16);
+                    if (key0 + key < it.keys) {
+                        acc = Pair16<T>::zero_times(u.x, acc);
+                        acc = Pair16<T>::zero_times(u.y, acc);
+                        acc = Pair16<T>::zero_times(u.z, acc);
+                        acc = Pair16<T>::zero_times(u.w, acc);
+                    }
                 }
-#pragma unroll
-                for (int n = 0; n < HD / 16; ++n) {
-                    unsigned r[4];
-                    const int key = ((lane >> 3) & 1) * 8 + (lane & 7), chunk = (n & 3) * 2 + (lane >> 4);
-                    ldmatrix4_trans(r, v_at + (b * kCols + (n >> 2)) * kBoxBytes + key * 128 + ((chunk ^ (key & 7)) << 4));
-                    if (tail) { r[0] &= keep0; r[1] &= keep1; r[2] &= keep0; r[3] &= keep1; }
-                    mma<T>(o[2 * n], w[b], r[0], r[1]);
-                    mma<T>(o[2 * n + 1], w[b], r[2], r[3]);
-                }
+                const float2 end = Pair16<T>::unpack(acc);
+                apart = __any_sync(0xffffffffu, end.x != end.x || end.y != end.y);
+            }
+            if (!apart) {
+                product<T, HD, false>(o, w, v_at, tail, it.keys - key0, true, true);
+            } else {
+                for (int token = 0; token < min(it.tokens, tile_tokens); ++token)
+                    product<T, HD, true>(o, w, v_at, true, it.seen + token + 1 - key0, seen[0] == it.seen + token, seen[1] == it.seen + token);
             }
             __syncwarp();                                       // all lanes have read the stage
             if (i + kStages < units) {
@@ -311,7 +356,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
 }
 
-constexpr CutRule kRule = {2, 1, 1, 1};
+constexpr CutRule kRule = {4, 1, 1, 2};
 
 template <typename T, int HD>
 int run(const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {

@@ -19,11 +19,14 @@
 // keeps small weights out of fp16's subnormal range.
 //
 // Keys behind a request's end are masked by index, whatever is stored there; their values would still meet a weight of
-// zero, so the product ends with the last key (in steps of 16, the rest of the last step cleared in shared memory).
+// zero, so the product ends with the last key (in steps of 16, the rest of the last step cleared in shared memory).  Where a
+// block holds keys that some of its rows do not see, its values are looked at: if one is not finite, the softmax threads form
+// that block's product themselves, each row over the keys it sees.
 //
 // TMEM: S/P of half 0 at column 0, of half 1 at 128; O of half 0 at 256, of half 1 at 256 + head_dim.
 
 #include <mutex>
+#include <type_traits>
 
 #include "attention_args.cuh"
 #include "attention_host.cuh"
@@ -128,6 +131,73 @@ __device__ __forceinline__ void swap_units(uint4& a, uint4& b, int lane) {
     if (upper) a = give; else b = give;
 }
 
+// Whether a half whose first row sees the keys up to `seen` does not see all of the block that begins with key0.
+__device__ __forceinline__ bool is_edge(int seen, int key0) { return seen + 1 - key0 < kKeyBlock; }
+
+// Whether any of the first `keys` rows of a slot of V holds an infinity or a NaN (0 x value is then a NaN); asked by the 128
+// threads of a half, who all get the answer.
+template <typename T, int HD>
+__device__ __forceinline__ bool any_not_finite(const unsigned char* v, int keys, int row, int barrier) {
+    unsigned acc = 0;                                           // two zeros, or NaN where something was not finite
+#pragma unroll
+    for (int x = 0; x < HD / 64; ++x)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = i * 128 + row;                       // 16-byte unit of the box, 8 to a key
+            if (at >> 3 >= keys) continue;
+            const uint4 u = *reinterpret_cast<const uint4*>(v + x * (128 * 128) + at * 16);
+            acc = Pair16<T>::zero_times(u.x, acc);
+            acc = Pair16<T>::zero_times(u.y, acc);
+            acc = Pair16<T>::zero_times(u.z, acc);
+            acc = Pair16<T>::zero_times(u.w, acc);
+        }
+    const float2 end = Pair16<T>::unpack(acc);
+    const bool bad = end.x != end.x || end.y != end.y;
+    unsigned any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(any) : "r"(static_cast<unsigned>(bad)), "r"(barrier) : "memory");
+    return any != 0;
+}
+
+// o += sum of p_k v_k over the first `keys` keys of a slot of V, by the row's own thread, p read back from tensor memory (o starts
+// anew if `fresh`).  Inline and without an array that is indexed at run time: a call, or a stack, in the kernel cost the
+// blocks that do not come here 10 %.
+template <typename T, int HD>
+__device__ __forceinline__ void product_by_hand(unsigned o_at, unsigned p_at, const unsigned char* v, int keys, bool fresh) {
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+        float o[32];
+        tmem_ld32(o_at + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = fresh ? 0.f : o[i];
+#pragma unroll 1
+        for (int k = 0; k < kKeyBlock; ++k) {
+            unsigned w2;
+            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(w2) : "r"(p_at + (k >> 1)) : "memory");
+            tmem_wait_ld();
+            const float2 both = Pair16<T>::unpack(w2);
+            const float w = k & 1 ? both.y : both.x;
+            const unsigned char* const at = v + (c >> 1) * (128 * 128) + k * 128;
+            if (k < keys) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(at + ((((c & 1) * 4 + i) ^ (k & 7)) << 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = Pair16<T>::unpack(e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w);
+                        o[i * 8 + 2 * e] = fmaf(w, f.x, o[i * 8 + 2 * e]);
+                        o[i * 8 + 2 * e + 1] = fmaf(w, f.y, o[i * 8 + 2 * e + 1]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        tmem_st32(o_at + c * 32, reinterpret_cast<const unsigned*>(o));
+    }
+    tmem_wait_st();
+}
+
 // An item and the blocks of keys that either half of its rows sees.
 struct HalvedItem {
     Item it;
@@ -179,6 +249,7 @@ struct Shared {
     unsigned long long k_full[kMaxSlots], k_empty[kMaxSlots], v_full[kMaxSlots], v_empty[kMaxSlots], item_full[kItems], item_empty[kItems];
     HalvedItem items[kItems];
     ShareScratch<kThreads> share;
+    int by_hand[2];                        // the block's product was formed by the softmax threads
     unsigned lost[kKeysSeen];              // 16-key groups of a block that are on no page of the cache
     unsigned tmem;
     int stop;
@@ -378,7 +449,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const HalvedItem& hit = sh.items[ring];
                 const int request = hit.it.request, blocks = hit.it.blocks;
                 const int count[2] = {hit.count[0], hit.count[1]};
-                const int keys = hit.it.keys - hit.it.block * kKeyBlock;
+                const int block0 = hit.it.block, keys = hit.it.keys - block0 * kKeyBlock;
+                const int seen_first[2] = {hit.it.seen, hit.it.seen + min(p.tokens_per_half, hit.it.tokens - 1)};
                 if (request < 0) break;
                 ++n_items;
                 for (int j = 0; j <= blocks && ok; ++j) {
@@ -388,7 +460,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     for (int h = 0; h < 2; ++h) {
                         const unsigned s_at = tmem + h * 128, o_at = tmem + 256 + h * HD;
                         if (j > 0 && j - 1 < count[h]) {
-                            const int live = min(kKeyBlock, max(0, keys - (j - 1) * kKeyBlock));
                             if (!v_here) {
                                 ok = warp_wait(smem_u32(&sh.v_full[v_slot]), (v_seq / kVSlots) & 1u, &sh.stop);
                                 if (!ok) break;
@@ -400,22 +471,32 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                                 ++o_count[h];
                             }
                             const uint64_t dv = v_desc + static_cast<uint64_t>((v_slot * kTile) >> 4);
+                            const unsigned more = j > 1;
+                            if (!is_edge(seen_first[h], (block0 + j - 1) * kKeyBlock)) {
 #pragma unroll
-                            for (int part = 0; part < 2; ++part) {      // P comes in two parts of 64 keys
-                                ok = warp_wait(smem_u32(&sh.p_full[h][part]), p_count[h] & 1u, &sh.stop);
-                                if (!ok) break;
-                                fence_after();
-                                if (elect_one()) {
-                                    if (live >= part * 64 + 64) {
+                                for (int part = 0; part < 2; ++part) {  // P comes in two parts of 64 keys
+                                    ok = warp_wait(smem_u32(&sh.p_full[h][part]), p_count[h] & 1u, &sh.stop);
+                                    if (!ok) break;
+                                    fence_after();
+                                    if (elect_one()) {
 #pragma unroll
                                         for (int k = part * 4; k < part * 4 + 4; ++k)
-                                            mma_tmem(o_at, s_at + k * 8, dv + ((k * 2048) >> 4), pv, j > 1 || k > 0);
-                                    } else {
-#pragma unroll 1
-                                        for (int k = part * 4; k * 16 < live; ++k)
-                                            mma_tmem(o_at, s_at + k * 8, dv + static_cast<uint64_t>((k * 2048) >> 4), pv, j > 1 || k > 0);
+                                            mma_tmem(o_at, s_at + k * 8, dv + ((k * 2048) >> 4), pv, k > 0 ? 1u : more);
+                                        if (part == 1 && j == count[h]) commit(smem_u32(&sh.o_full[h]));
                                     }
-                                    if (part == 1 && j == count[h]) commit(smem_u32(&sh.o_full[h]));
+                                    __syncwarp();
+                                }
+                            } else {
+                                const int live = min(kKeyBlock, max(0, keys - (j - 1) * kKeyBlock));
+                                ok = warp_wait(smem_u32(&sh.p_full[h][0]), p_count[h] & 1u, &sh.stop) && warp_wait(smem_u32(&sh.p_full[h][1]), p_count[h] & 1u, &sh.stop);
+                                if (!ok) break;
+                                fence_after();
+                                const bool by_hand = *static_cast<volatile int*>(&sh.by_hand[h]) != 0;
+                                if (elect_one()) {
+#pragma unroll 1
+                                    for (int k = 0; k * 16 < live && !by_hand; ++k)
+                                        mma_tmem(o_at, s_at + k * 8, dv + static_cast<uint64_t>((k * 2048) >> 4), pv, k > 0 ? 1u : more);
+                                    if (j == count[h]) commit(smem_u32(&sh.o_full[h]));
                                 }
                                 __syncwarp();
                             }
@@ -480,33 +561,18 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             ++n_items;
             const bool live_row = in_tile && token < it.tokens;
             const int seen = it.seen + min(token, it.tokens - 1);              // the last key this row sees
+            const int seen_first = it.seen + min(h * p.tokens_per_half, it.tokens - 1);      // and the half's first row
             float top = -INFINITY, bias = 0.f, sum = 0.f;                       // maximum of s; exponent = s * scale - bias
-            for (int j = 0; j < count && ok; ++j) {
-                ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
-                if (!ok) break;
-                ++s_count;
-                fence_after();
+            // One block of keys.  `Edge` where its rows do not all see all of its keys; apart, so that the registers and the schedule of
+            // the others, which are nearly all, do not pay for it.
+            auto block = [&](auto edge, int j, int key0, unsigned lost, bool by_hand) {
+                constexpr bool kEdge = decltype(edge)::value;
                 float s[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, s + c * 32);
                 tmem_wait_ld();
-                const int key0 = (it.block + j) * kKeyBlock;
                 const int allowed = seen + 1 - key0;
-                const unsigned lost = PAGED ? sh.lost[(block_seq + j) % kKeysSeen] : 0u;
-                const int rest = it.keys - key0;                               // keys that exist, from this block's first on
-                if (rest < kKeyBlock && (rest & 15) != 0) {
-                    // What lies behind the last key may be anything; its weight is zero, and zero times it must be too.  The
-                    // product ends with the last key's 16: clear the rest of those in V.
-                    const int slot = (block_seq + j) % kVSlots;
-                    ok = warp_wait(smem_u32(&sh.v_full[slot]), ((block_seq + j) / kVSlots) & 1u, &sh.stop);
-                    if (!ok) break;
-                    const int gone = rest > 0 ? 16 - (rest & 15) : 0;
-                    unsigned char* const v = v_tiles + slot * kTile + rest * 128;
-                    for (int i = row; i < gone * 8 * kBoxes; i += 128)
-                        *reinterpret_cast<uint4*>(v + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                if (__any_sync(0xffffffffu, allowed < kKeyBlock) || (PAGED && lost != 0)) {
+                if constexpr (kEdge) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
                         if (i >= allowed || (PAGED && ((lost >> (i / 16)) & 1u))) s[i] = -INFINITY;
@@ -540,6 +606,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                 }
+                if (kEdge && lane == 0) sh.by_hand[h] = by_hand;
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), bias2 = make_float2(-bias, -bias);
                 float2 part[4];
 #pragma unroll
@@ -554,12 +621,42 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     tmem_st32(s_at + c * 32, w);
                     tmem_wait_st();
+                    if constexpr (kEdge) {
+                        if (c == 1 && by_hand) product_by_hand<T, HD>(o_at, s_at, v_tiles + (block_seq + j) % kVSlots * kTile, allowed, j == 0);
+                    }
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[h][c]));
                 }
                 const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
                 sum += all.x + all.y;
+            };
+            for (int j = 0; j < count && ok; ++j) {
+                const int key0 = (it.block + j) * kKeyBlock;
+                const bool edge = is_edge(seen_first, key0);
+                bool by_hand = false;
+                if (edge) {                                    // while the scores are formed: what stands in V behind the keys seen
+                    const int slot = (block_seq + j) % kVSlots, rest = it.keys - key0;
+                    ok = warp_wait(smem_u32(&sh.v_full[slot]), ((block_seq + j) / kVSlots) & 1u, &sh.stop);
+                    if (!ok) break;
+                    unsigned char* const v = v_tiles + slot * kTile;
+                    if (rest < kKeyBlock && (rest & 15) != 0) {
+                        // What lies behind the last key may be anything; its weight is zero, and zero times it must be too.  The
+                        // product ends with the last key's 16: clear the rest of those.
+                        const int gone = rest > 0 ? 16 - (rest & 15) : 0;
+                        for (int i = row; i < gone * 8 * kBoxes; i += 128)
+                            *reinterpret_cast<uint4*>(v + rest * 128 + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    if (seen_first + 1 - key0 < min(rest, kKeyBlock)) by_hand = any_not_finite<T, HD>(v, rest, row, 1 + h);
+                }
+                ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
+                if (!ok) break;
+                ++s_count;
+                fence_after();
+                const unsigned lost = PAGED ? sh.lost[(block_seq + j) % kKeysSeen] : 0u;
+                if (edge || (PAGED && lost != 0)) block(std::true_type{}, j, key0, lost, by_hand);
+                else block(std::false_type{}, j, key0, 0u, false);
             }
             block_seq += it.blocks;
             if (!ok) break;
@@ -633,7 +730,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
-constexpr CutRule kRule = {8, 2, 1, 1};
+constexpr CutRule kRule = {12, 2, 1, 2};
 template <typename T, int HD, bool PAGED>
 int run(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttentionArgs& args, int dev, cudaStream_t stream) {
     static std::once_flag once[64];

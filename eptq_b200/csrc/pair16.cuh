@@ -16,6 +16,11 @@ struct Pair16<__half> {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const unsigned*>(&h);
     }
+    // 0 * w + acc: NaN where w is not finite.
+    static __device__ __forceinline__ unsigned zero_times(unsigned w, unsigned acc) {
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w), "r"(0u));
+        return acc;
+    }
 };
 
 template <>
@@ -24,6 +29,10 @@ struct Pair16<__nv_bfloat16> {
     static __device__ __forceinline__ unsigned pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const unsigned*>(&h);
+    }
+    static __device__ __forceinline__ unsigned zero_times(unsigned w, unsigned acc) {
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w), "r"(0u));
+        return acc;
     }
 };
 

@@ -237,6 +237,29 @@ def test_paged_attention_strided_q():
         check(_attend(s, max_rows=told), want, tol)
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("nh,nkv,hd,lens,told", [(8, 2, 128, [(300, 40)], 100000), (4, 4, 64, [(513, 300), (70, 2)], 100000), (8, 2, 128, [(90, 4), (33, 2)], 4),
+                                                 (6, 2, 64, [(64, 5)], 5), (7, 1, 128, [(1500, 140)], 100000)])
+def test_paged_attention_values_not_finite(dtype, nh, nkv, hd, lens, told):
+    """A value that is not finite reaches the rows that see it, in its column, and no other row: not the request's earlier ones."""
+    s = make_step(lens, nh, nkv, hd, 16, dtype, seed=12)
+    want, tol = step_reference(s, nh)
+    want, tol = want.reshape(-1, nh, hd).clone(), tol.reshape(-1, nh, hd)
+    at = 0
+    for b, (kv, n) in enumerate(lens):
+        for key, col, head, value in ((kv - n + 1, 3, 0, float("inf")), (kv - 1, 5, nkv - 1, float("nan")), (kv - (n + 1) // 2, hd - 1, 0, float("-inf"))):
+            page = int(s["tables"][b, key // 16])
+            s["v_cache"][page, head, key % 16, col] = value
+            rows = slice(at + key - (kv - n), at + n)
+            want[rows, head * (nh // nkv):(head + 1) * (nh // nkv), col] += value
+        at += n
+    out = _attend(s, max_rows=told).double().reshape(-1, nh, hd)
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), finite)
+    assert bool((((out - want).abs() <= tol) | ~finite).all())
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool((out[~finite & ~torch.isnan(want)] == want[~finite & ~torch.isnan(want)]).all())
+
+
 # ---- packed prompts --------------------------------------------------------------------------------------------
 def _prompt_reference(q, k, v, lens, nh, nkv, hd, scale=None):
     outs, tols, at = [], [], 0
