@@ -100,9 +100,11 @@ __device__ __forceinline__ void tma_4d(unsigned dst, const CUtensorMap* map, int
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
 
+// (Plain loads here and wherever a kernel reads what the one before it may have written: it may start before that one has
+// ended, and a read-only load may be served from before its own wait.)
 __device__ __forceinline__ Request load_request(const AttentionArgs& p, int b) {
     const bool paged = p.page_size != 0;
-    return request_from(__ldg(p.cu_rows + b), __ldg(p.cu_rows + b + 1), p.rows, paged ? __ldg(p.kv_lens + b) : 0, p.table_keys, paged);
+    return request_from(p.cu_rows[b], p.cu_rows[b + 1], p.rows, paged ? p.kv_lens[b] : 0, p.table_keys, paged);
 }
 
 // The part of the work that falls to one block of the launch.

@@ -142,7 +142,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int sub = kSub == 2 ? lane & 1 : 0, col64 = kSub == 2 ? 0 : lane & 1;
         auto page_of = [&](int i) {                        // page of this lane's box of unit i
             const int key = (unit0 + i * kWarps) * kUnit + sub * 16;
-            return lane < 4 && i < units && key < it.keys ? __ldg(table + (key >> page_shift)) : 0;
+            return lane < 4 && i < units && key < it.keys ? table[key >> page_shift] : 0;
         };
         unsigned lost = 0;                                 // two bits a stage: 16-key groups on no page of the cache
         auto load = [&](int i, int page) {
@@ -180,7 +180,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                    q[k][2 * c + e] = live ? __ldg(reinterpret_cast<const unsigned*>(src + k * 16 + c * 8)) : 0u;
+                    q[k][2 * c + e] = live ? *reinterpret_cast<const unsigned*>(src + k * 16 + c * 8) : 0u;
         }
         float o[HD / 8][4], top[2], bias[2], sum[2];
 #pragma unroll

@@ -134,10 +134,10 @@ __device__ __forceinline__ void swap_units(uint4& a, uint4& b, int lane) {
 // Whether a half whose first row sees the keys up to `seen` does not see all of the block that begins with key0.
 __device__ __forceinline__ bool is_edge(int seen, int key0) { return seen + 1 - key0 < kKeyBlock; }
 
-// Whether any of the first `keys` rows of a slot of V holds an infinity or a NaN (0 x value is then a NaN); asked by the 128
-// threads of a half, who all get the answer.
+// Whether any of the first `keys` rows of a slot of V holds an infinity or a NaN (0 x value is then a NaN): one warp's part of
+// what the 128 threads of a half look at.
 template <typename T, int HD>
-__device__ __forceinline__ bool any_not_finite(const unsigned char* v, int keys, int row, int barrier) {
+__device__ __forceinline__ bool any_not_finite(const unsigned char* v, int keys, int row) {
     unsigned acc = 0;                                           // two zeros, or NaN where something was not finite
 #pragma unroll
     for (int x = 0; x < HD / 64; ++x)
@@ -152,11 +152,7 @@ __device__ __forceinline__ bool any_not_finite(const unsigned char* v, int keys,
             acc = Pair16<T>::zero_times(u.w, acc);
         }
     const float2 end = Pair16<T>::unpack(acc);
-    const bool bad = end.x != end.x || end.y != end.y;
-    unsigned any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(any) : "r"(static_cast<unsigned>(bad)), "r"(barrier) : "memory");
-    return any != 0;
+    return __any_sync(0xffffffffu, end.x != end.x || end.y != end.y);
 }
 
 // o += sum of p_k v_k over the first `keys` keys of a slot of V, by the row's own thread, p read back from tensor memory (o starts
@@ -215,7 +211,7 @@ struct PageRow {
         const int shift = 31 - __clz(p.page_size), at = key0 >> shift, n = (max(0, keys) + p.page_size - 1) >> shift;
         if (column < 0 || at + n > column + 32) {
             column = at;
-            id = at + lane < p.table_width ? __ldg(p.tables + request * p.table_stride + at + lane) : -1;
+            id = at + lane < p.table_width ? p.tables[request * p.table_stride + at + lane] : -1;
         }
         page = __shfl_sync(0xffffffffu, id, (at - column + lane) & 31);
         if (page < 0 || page >= p.n_pages) page = p.n_pages;
@@ -249,6 +245,8 @@ struct Shared {
     unsigned long long k_full[kMaxSlots], k_empty[kMaxSlots], v_full[kMaxSlots], v_empty[kMaxSlots], item_full[kItems], item_empty[kItems];
     HalvedItem items[kItems];
     ShareScratch<kThreads> share;
+    unsigned long long voted[2];
+    int votes[2][4];                       // ring: a half's block holds a value that is not finite
     int by_hand[2];                        // the block's product was formed by the softmax threads
     unsigned lost[kKeysSeen];              // 16-key groups of a block that are on no page of the cache
     unsigned tmem;
@@ -279,6 +277,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(smem_u32(&sh.p_full[h][1]), 4);
             mbar_init(smem_u32(&sh.o_full[h]), 1);
             mbar_init(smem_u32(&sh.o_empty[h]), 4);
+            mbar_init(smem_u32(&sh.voted[h]), 4);
+            for (int i = 0; i < 4; ++i) sh.votes[h][i] = 0;
         }
         for (int s = 0; s < kMaxSlots; ++s) {
             mbar_init(smem_u32(&sh.k_full[s]), 1);
@@ -550,7 +550,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const unsigned s_at = tmem + lanes + h * 128, o_at = tmem + lanes + 256 + h * HD;
         const int token = h * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
         const bool in_tile = row < p.heads_per_tile * p.tokens_per_half;
-        unsigned n_items = 0, s_count = 0, o_count = 0, block_seq = 0;
+        unsigned n_items = 0, s_count = 0, o_count = 0, block_seq = 0, vote = 0;
         while (ok) {
             const int ring = n_items % kItems;
             ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
@@ -648,7 +648,20 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             *reinterpret_cast<uint4*>(v + rest * 128 + (i / (gone * 8)) * kBox + (i % (gone * 8)) * 16) = make_uint4(0, 0, 0, 0);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
-                    if (seen_first + 1 - key0 < min(rest, kKeyBlock)) by_hand = any_not_finite<T, HD>(v, rest, row, 1 + h);
+                    if (seen_first + 1 - key0 < min(rest, kKeyBlock)) {
+                        // The half's four warps agree by a bounded wait like all others.  Two entries on, the ring is cleared: whoever is
+                        // past the last vote knows that all have read the one before it.
+                        const bool bad = any_not_finite<T, HD>(v, rest, row);
+                        if (lane == 0) {
+                            sh.votes[h][(vote + 2) & 3] = 0;
+                            if (bad) sh.votes[h][vote & 3] = 1;
+                            mbar_arrive(smem_u32(&sh.voted[h]));
+                        }
+                        ok = warp_wait(smem_u32(&sh.voted[h]), vote & 1u, &sh.stop);
+                        if (!ok) break;
+                        by_hand = *static_cast<volatile int*>(&sh.votes[h][vote & 3]) != 0;
+                        ++vote;
+                    }
                 }
                 ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
                 if (!ok) break;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanArgs
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, ps = p.page_size;
-    const long long n_free = min(max(__ldg(p.n_free), 0), p.free_cap);
+    const long long n_free = min(max(*p.n_free, 0), p.free_cap);
     const bool first_block = blockIdx.x == 0;
     const long long step = static_cast<long long>(gridDim.x) * kPlanThreads;
     if (tid == 0) taken = 0;

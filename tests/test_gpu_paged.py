@@ -444,7 +444,9 @@ def test_nothing_to_do():
     out = torch.full((2, 256), 5.0, dtype=FP16, device="cuda")
     paged.paged_attention(torch.zeros_like(out), cache, cache, i(0, 5), i(0), i(1), 1, out=out)
     assert bool((out == 5).all())
-    paged.paged_attention(torch.zeros_like(out), cache[:0], cache[:0], i(1, 0), i(1) + 9, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), 2, out=out)
-    assert bool((out == 0).all())
+    for told in (2, 1000):                                                 # a cache without pages
+        out.fill_(5)
+        paged.paged_attention(torch.zeros_like(out), cache[:0], cache[:0], i(1, 0), i(1) + 9, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), told, out=out)
+        assert bool((out == 0).all())
     assert paged.prompt_attention(e(0, 256), e(0, 128), e(0, 128), i(1), 64).shape == (0, 256)
     assert paged.rope_append_paged(e(0, 256), e(0, 128), e(0, 128), cache, cache, e(0, dtype=torch.int64), e(0, dtype=torch.int64), e(32, dtype=torch.float32)).shape == (0, 256)
