@@ -99,6 +99,14 @@ at::Tensor output(PyObject* o, const at::Tensor& q) {
     return out;
 }
 
+// `n` values of `type` from the `at`-th on in the storage of `all`, as a tensor of its own.
+at::Tensor part(const at::Tensor& all, at::ScalarType type, int64_t at, int64_t n) {
+    auto t = c10::make_intrusive<at::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+    t->set_storage_offset(at);
+    t->set_sizes_contiguous({n});
+    return at::Tensor(std::move(t));
+}
+
 void done(int status, const char* what) { TORCH_CHECK(status == EPTQ_OK, "eptq ", what, ": ", eptq_strerror(status), " (eptq status ", status, ")"); }
 
 void arguments(Py_ssize_t n, Py_ssize_t want, const char* usage) { TORCH_CHECK_TYPE(n == want, usage); }
@@ -136,8 +144,10 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     REFUSE_UNLESS(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "page_size must be 16, 32, 64 or 128");
     REFUSE_UNLESS(rows >= 0, "rows must not be negative");
     const c10::cuda::OptionalCUDAGuard guard(device);
-    const auto i32 = cached.options(), i64 = i32.dtype(at::kLong);
-    at::Tensor out[5] = {at::empty({B + 1}, i32), at::empty({B}, i32), at::empty({rows}, i64), at::empty({rows}, i64), at::empty({1}, i32)};
+    // One allocation for the five outputs, each a part of it: five cost more than the kernel.
+    const at::Tensor all = at::empty({2 * rows + B + 1}, cached.options().dtype(at::kLong));
+    at::Tensor out[5] = {part(all, at::kInt, 4 * rows, B + 1), part(all, at::kInt, 4 * rows + B + 1, B), part(all, at::kLong, 0, rows),
+                         part(all, at::kLong, rows, rows), part(all, at::kInt, 4 * rows + 2 * B + 1, 1)};
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
     done(eptq_plan_pages(cached.const_data_ptr<int32_t>(), fresh.const_data_ptr<int32_t>(), batch, const_cast<int32_t*>(tables.const_data_ptr<int32_t>()), stride, width,
                          free_pages.const_data_ptr<int32_t>(), cap, n_free.const_data_ptr<int32_t>(), page_size, n_rows, out[0].data_ptr<int32_t>(),
