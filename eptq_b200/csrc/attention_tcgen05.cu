@@ -13,10 +13,14 @@
 //               the other half's softmax runs.
 //   warps 4-11  softmax, one thread per row and half: S from TMEM, maximum, exp2, P back to TMEM in 16 bits.
 //
-// Per 128 x 128 half-block the tensor core needs 1024 cycles (head 128) and the exponentials 1024 cycles of the SM's
-// special-function units: the two bound the kernel together.  O is rescaled only when a row's maximum has grown by more
-// than 2^8, by the softmax thread itself; P then stays below 2^15 because exponents carry an offset of 7, which also
-// keeps small weights out of fp16's subnormal range.
+// Per 128 x 128 half-block (head 128) the tensor cores need 1024 cycles and the exponentials 1024 cycles of the SM's
+// special-function units.  What bounds the kernel is the chain of one half: 2100 cycles of softmax, one warp's instructions one
+// after the other, then 1200 until the next scores are there; two halves in turn keep the tensor cores busy 60 % of the time.
+// O is rescaled only when a row's maximum has grown by more than 2^8, by the softmax thread itself; P then stays below
+// 2^15 because exponents carry an offset of 7, which also keeps small weights out of fp16's subnormal range.
+//
+// Measured on one B200: prompt of 16384 tokens, 32 over 8 heads of 128, 1.77 ms (1240 TFLOP/s); 8191 tokens, 32 heads, 523 us
+// (1050 TFLOP/s); 509 rows of 64 over 8 heads on 24001 keys 389 us (1040 TFLOP/s); 1024 tokens 26 us.
 //
 // Keys behind a request's end are masked by index, whatever is stored there; their values would still meet a weight of
 // zero, so the product ends with the last key (in steps of 16, the rest of the last step cleared in shared memory).  Where a
