@@ -106,3 +106,16 @@ def test_plan_reference_by_hand():
     assert slots == [16, 17, 37, 38, 39] + [144 + i for i in range(16)] + [112 + i for i in range(4)] + [-1] * 5
     tables, cu, kv, pos, slots, left = plan_reference([16, 5, 0], [2, 3, 20], [[4, -1], [2, -1], [-1, -1]], [7, 9], 2, 16, 25)
     assert kv == [18, 8, 0] and left == 1 and slots[5:] == [-1] * 20
+
+
+def test_schedule_takes_every_block_once(tmp_path):
+    """The device's schedule, compiled for the host: shares of random calls cover the work once, cut tiles know their pieces."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    source = Path(__file__).with_name("schedule_check.cpp")
+    program = tmp_path / "schedule_check"
+    subprocess.run([shutil.which("g++") or "g++", "-O1", "-std=c++17", "-o", str(program), str(source)], check=True)
+    out = subprocess.run([str(program)], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout
+    assert int(out.stdout.split()[1]) > 10000
