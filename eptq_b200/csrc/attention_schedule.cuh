@@ -180,4 +180,22 @@ EPTQ_HD int last_share(long long tile_end, long long share, const CutRule& rule)
     return static_cast<int>(quotient(tile_end - rule.near + share - 1, share)) - 1;
 }
 
+// ---- a row tile in two halves of tokens, which take turns ----
+
+// Blocks of an item (the tile's blocks `block` .. block + blocks - 1) that each half takes part in, from the first on: half 0 sees
+// fewer keys than half 1, and a half without tokens has no blocks.
+EPTQ_HD void half_blocks(int seen, int tokens, int tokens_per_half, int kb, int block, int blocks, int (&count)[2]) {
+    const int keys0 = seen + (tokens < tokens_per_half ? tokens : tokens_per_half);
+    const int need0 = keys0 <= kb ? 1 : (keys0 + kb - 1) / kb, left0 = need0 - block;
+    count[0] = left0 < 0 ? 0 : left0 < blocks ? left0 : blocks;
+    count[1] = tokens > tokens_per_half ? blocks : 0;
+}
+
+// Whether a half waits for the scores of an item's block j before it waits for the block's values.  A wait by parity tells only
+// neighbouring fills of a ring's slot apart, so whoever waits for a fill has to know that the one before it has landed.  A half that
+// took part in the block before knows it of all values but that block's: its last scores were formed behind them.  One that sat out
+// blocks of the item before (all of them, where it has no tokens) may be any number of fills behind, and knows it only from the scores of
+// its own next block, which are formed behind all earlier values.
+EPTQ_HD bool scores_before_values(bool sat_out, int j) { return sat_out && j == 0; }
+
 }  // namespace eptq

@@ -342,11 +342,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     break;
                 }
-                // half 0 sees fewer keys than half 1; a half without tokens has no blocks
-                const int keys0 = it.seen + min(it.tokens, p.tokens_per_half);
-                const int need0 = keys0 <= kKeyBlock ? 1 : (keys0 + kKeyBlock - 1) / kKeyBlock;
-                hit.count[0] = max(0, min(it.blocks, need0 - it.block));
-                hit.count[1] = it.tokens > p.tokens_per_half ? it.blocks : 0;
+                half_blocks(it.seen, it.tokens, p.tokens_per_half, kKeyBlock, it.block, it.blocks, hit.count);
                 hit.first = walk.r.first;
                 if (elect_one()) {
                     sh.items[ring] = hit;
@@ -555,6 +551,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int token = h * p.tokens_per_half + row / p.heads_per_tile, head = row % p.heads_per_tile;
         const bool in_tile = row < p.heads_per_tile * p.tokens_per_half;
         unsigned n_items = 0, s_count = 0, o_count = 0, block_seq = 0, vote = 0;
+        bool sat_out = false;                                                   // blocks of the item before
         while (ok) {
             const int ring = n_items % kItems;
             ok = warp_wait(smem_u32(&sh.item_full[ring]), (n_items / kItems) & 1u, &sh.stop);
@@ -638,7 +635,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int j = 0; j < count && ok; ++j) {
                 const int key0 = (it.block + j) * kKeyBlock;
                 const bool edge = is_edge(seen_first, key0);
+                const bool scores_first = scores_before_values(sat_out, j);
                 bool by_hand = false;
+                if (scores_first) {
+                    ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
+                    if (!ok) break;
+                }
                 if (edge) {                                    // while the scores are formed: what stands in V behind the keys seen
                     const int slot = (block_seq + j) % kVSlots, rest = it.keys - key0;
                     ok = warp_wait(smem_u32(&sh.v_full[slot]), ((block_seq + j) / kVSlots) & 1u, &sh.stop);
@@ -667,8 +669,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         ++vote;
                     }
                 }
-                ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
-                if (!ok) break;
+                if (!scores_first) {
+                    ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
+                    if (!ok) break;
+                }
                 ++s_count;
                 fence_after();
                 const unsigned lost = PAGED ? sh.lost[(block_seq + j) % kKeysSeen] : 0u;
@@ -676,6 +680,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 else block(std::false_type{}, j, key0, 0u, false);
             }
             block_seq += it.blocks;
+            sat_out = count < it.blocks;
             if (!ok) break;
             if (count > 0) {
                 ok = warp_wait(smem_u32(&sh.o_full[h]), o_count & 1u, &sh.stop);
