@@ -191,11 +191,11 @@ EPTQ_HD void half_blocks(int seen, int tokens, int tokens_per_half, int kb, int 
     count[1] = tokens > tokens_per_half ? blocks : 0;
 }
 
-// Whether a half waits for the scores of an item's block j before it waits for the block's values.  A wait by parity tells only
-// neighbouring fills of a ring's slot apart, so whoever waits for a fill has to know that the one before it has landed.  A half that
-// took part in the block before knows it of all values but that block's: its last scores were formed behind them.  One that sat out
-// blocks of the item before (all of them, where it has no tokens) may be any number of fills behind, and knows it only from the scores of
-// its own next block, which are formed behind all earlier values.
-EPTQ_HD bool scores_before_values(bool sat_out, int j) { return sat_out && j == 0; }
+// Whether a half that takes part in `count` blocks of an item waits for the scores of the first before it waits for any values.  A wait by
+// parity tells only neighbouring fills of a ring's slot apart, so whoever waits for a fill has to know that the one before it has
+// landed.  A half that took part in the block before knows it of all values but that block's: its last scores were formed behind them.  One
+// that sat out blocks of the item before (all of them, where it has no tokens) may be any number of fills behind, and knows it only
+// from the scores of its own next block, which are formed behind all earlier values.
+EPTQ_HD bool scores_before_values(bool sat_out, int count) { return sat_out && count > 0; }
 
 }  // namespace eptq

@@ -632,15 +632,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
                 sum += all.x + all.y;
             };
+            // (the first block waits for them again, and goes on at once)
+            if (scores_before_values(sat_out, count)) ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
             for (int j = 0; j < count && ok; ++j) {
                 const int key0 = (it.block + j) * kKeyBlock;
                 const bool edge = is_edge(seen_first, key0);
-                const bool scores_first = scores_before_values(sat_out, j);
                 bool by_hand = false;
-                if (scores_first) {
-                    ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
-                    if (!ok) break;
-                }
                 if (edge) {                                    // while the scores are formed: what stands in V behind the keys seen
                     const int slot = (block_seq + j) % kVSlots, rest = it.keys - key0;
                     ok = warp_wait(smem_u32(&sh.v_full[slot]), ((block_seq + j) / kVSlots) & 1u, &sh.stop);
@@ -669,10 +666,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         ++vote;
                     }
                 }
-                if (!scores_first) {
-                    ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
-                    if (!ok) break;
-                }
+                ok = warp_wait(smem_u32(&sh.s_full[h]), s_count & 1u, &sh.stop);
+                if (!ok) break;
                 ++s_count;
                 fence_after();
                 const unsigned lost = PAGED ? sh.lost[(block_seq + j) % kKeysSeen] : 0u;

@@ -38,8 +38,7 @@ int main() {
             }
             for (int h = 0; h < 2; ++h) {
                 for (int j = 0; j < count[h]; ++j) {
-                    const bool first = scores_before_values(sat_out[h], j);
-                    if (first) known[h] = std::max(known[h], base + j - 1);
+                    if (j == 0 && scores_before_values(sat_out[h], count[h])) known[h] = std::max(known[h], base - 1);
                     if (base + j - ring > known[h]) {
                         std::printf("walk %d, item %d, half %d: waits for block %lld in %d slots and knows of block %lld\n", walk, item, h, base + j, ring, known[h]);
                         return 1;
