@@ -607,7 +607,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                 }
-                if (kEdge && lane == 0) sh.by_hand[h] = by_hand;
+                if constexpr (kEdge) {
+                    if (lane == 0) sh.by_hand[h] = by_hand;
+                    __syncwarp();
+                }
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), bias2 = make_float2(-bias, -bias);
                 float2 part[4];
 #pragma unroll
@@ -628,6 +631,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[h][c]));
+                    if (c == 0) __syncwarp();                       // the next tcgen05.st wants the whole warp
                 }
                 const float2 all = add2(add2(part[0], part[1]), add2(part[2], part[3]));
                 sum += all.x + all.y;
@@ -709,6 +713,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (at[r] >= 0) *reinterpret_cast<uint4*>(p.out + at[r] + c * 32 + (lane & 3) * 8) = u[r];
+                        __syncwarp();                               // the next tcgen05.ld wants the whole warp
                     }
                 }
             } else if (it.tokens > h * p.tokens_per_half) {
@@ -722,10 +727,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         float o[32];
                         tmem_ld32(o_at + c * 32, o);
                         tmem_wait_ld();
-                        if (!live_row) continue;
+                        if (live_row) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            reinterpret_cast<float4*>(piece)[(c * 8 + i) * 256 + at_row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            for (int i = 0; i < 8; ++i)
+                                reinterpret_cast<float4*>(piece)[(c * 8 + i) * 256 + at_row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                        __syncwarp();                               // the next tcgen05.ld wants the whole warp
                     }
                 }
             }
