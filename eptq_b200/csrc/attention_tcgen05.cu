@@ -255,6 +255,7 @@ struct Shared {
     unsigned lost[kKeysSeen];              // 16-key groups of a block that are on no page of the cache
     unsigned tmem;
     int stop;
+    unsigned long long drained;
 };
 
 template <typename T, int HD, bool PAGED>
@@ -294,6 +295,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(smem_u32(&sh.item_full[s]), 1);
             mbar_init(smem_u32(&sh.item_empty[s]), 10);
         }
+        mbar_init(smem_u32(&sh.drained), 1);
         sh.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&map_q)) : "memory");
@@ -539,6 +541,14 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 __syncwarp();
                 if (elect_one()) mbar_arrive(smem_u32(&sh.item_empty[ring]));
+            }
+            if (!ok) {
+                // products still in flight read shared memory and write tensor memory: wait for them before both are given up
+                volatile int never = 0;
+                __syncwarp();
+                if (elect_one()) commit(smem_u32(&sh.drained));
+                __syncwarp();
+                warp_wait(smem_u32(&sh.drained), 0, &never);
             }
         }
     } else {
