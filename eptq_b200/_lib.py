@@ -99,7 +99,7 @@ class EptqAttention(C.Structure):
         ("dtype", C.c_int32), ("rows", C.c_int32), ("batch", C.c_int32),
         ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("max_rows", C.c_int32),
         ("page_size", C.c_int32), ("n_pages", C.c_int32), ("table_width", C.c_int32),
-        ("scale", C.c_float), ("reserved", C.c_int32),
+        ("scale", C.c_float), ("clear_rest", C.c_int32),
         ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("table_stride", C.c_int64),
         ("q", _vp), ("k", _vp), ("v", _vp), ("tables", _vp), ("kv_lens", _vp), ("cu_rows", _vp), ("out", _vp),
         ("status", _vp),

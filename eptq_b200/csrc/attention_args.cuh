@@ -31,6 +31,7 @@ struct AttentionArgs {
     int page_size, n_pages, table_width;
     float scale_log2;              // |scale| * log2(e)
     int negative;                  // scale is below zero
+    int clear_rest;                // rows of no request become zeros
 };
 
 // A piece of a cut tile: o [head_dim / 4][tile_rows][4], then the exponent's reference and the sum of each row, fp32.  Rows whose
@@ -105,6 +106,16 @@ __device__ __forceinline__ void tma_4d(unsigned dst, const CUtensorMap* map, int
 __device__ __forceinline__ Request load_request(const AttentionArgs& p, int b) {
     const bool paged = p.page_size != 0;
     return request_from(p.cu_rows[b], p.cu_rows[b + 1], p.rows, paged ? p.kv_lens[b] : 0, p.table_keys, paged);
+}
+
+// The rows ahead of the first request and behind the last one become zeros, 16 bytes a thread.  Not inline: the registers it would take
+// cost the kernel of few rows 4 % where a call has nothing to clear.
+template <int kThreads, int HD>
+__device__ __noinline__ void clear_rest(const AttentionArgs& p) {
+    const long long row = static_cast<long long>(p.n_heads) * (HD / 8), first = min(max(p.cu_rows[0], 0), p.rows) * row;
+    const long long end = min(max(p.cu_rows[p.batch], 0), p.rows) * row, rest = first + p.rows * row - end;
+    for (long long i = blockIdx.x * kThreads + threadIdx.x; i < rest; i += gridDim.x * kThreads)
+        reinterpret_cast<uint4*>(p.out)[i < first ? i : end + i - first] = make_uint4(0, 0, 0, 0);
 }
 
 // The part of the work that falls to one block of the launch.

@@ -351,6 +351,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the stages are written by TMA again
         __syncthreads();
     }
+    if (p.clear_rest) clear_rest<kThreads, HD>(p);
     if (tid == 0 && !cut_written && p.cut_tiles != nullptr) p.cut_tiles[blockIdx.x].of = 0;
     if (!ok) {
         // copies still in flight write shared memory: wait for them before it is given up

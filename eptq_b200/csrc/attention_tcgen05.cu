@@ -305,6 +305,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
+    if (p.clear_rest) clear_rest<kThreads, HD>(p);
     const Share share = find_share<kThreads, 1>(p, tile_tokens, kKeyBlock, rule, sh.share);
     if (share.begin >= share.end) {                                // nothing left for this block
         if (tid == 0 && p.cut_tiles != nullptr) p.cut_tiles[blockIdx.x].of = 0;

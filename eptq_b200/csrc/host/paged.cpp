@@ -199,6 +199,7 @@ PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const 
     const c10::Device device = q.device();
     const c10::cuda::OptionalCUDAGuard guard(device);
     at::Tensor out = output(out_or_none, q);
+    a.clear_rest = out_or_none == Py_None;          // memory of the allocator's: rows of no request would show what it held
     a.rows = narrow(q.size(0), "the number of rows");
     a.batch = narrow(cu_rows.numel() - 1, "the number of requests");
     a.scale = static_cast<float>(scale == Py_None ? 1.0 / std::sqrt(static_cast<double>(a.head_dim)) : number(scale));

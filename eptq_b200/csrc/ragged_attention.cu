@@ -133,6 +133,7 @@ int check(const EptqAttention& a) {
                   a.table_stride < a.table_width)) return EPTQ_ERR_SHAPE;
     const int64_t kv_row = static_cast<int64_t>(a.n_kv_heads) * a.head_dim * (paged ? a.page_size : 1);
     if (a.q_stride < static_cast<int64_t>(a.n_heads) * a.head_dim || a.k_stride < kv_row || a.v_stride < kv_row) return EPTQ_ERR_SHAPE;
+    if (a.rows > 0 && a.clear_rest != 0 && a.out == nullptr) return EPTQ_ERR_NULL;
     if (a.rows > 0 && a.batch > 0 && (a.q == nullptr || a.out == nullptr || a.cu_rows == nullptr ||
                                       (paged && (a.kv_lens == nullptr || (a.tables == nullptr && a.table_width > 0))) ||
                                       ((!paged || a.n_pages > 0) && (a.k == nullptr || a.v == nullptr)))) return EPTQ_ERR_NULL;
@@ -172,7 +173,11 @@ extern "C" int eptq_ragged_attention(const EptqAttention* args, void* workspace,
     if (args == nullptr) return EPTQ_ERR_NULL;
     const EptqAttention& a = *args;
     if (const int st = check(a); st != EPTQ_OK) return st;
-    if (a.rows == 0 || a.batch == 0) return EPTQ_OK;
+    if (a.rows == 0) return EPTQ_OK;
+    if (a.batch == 0) {
+        const size_t bytes = static_cast<size_t>(a.rows) * a.n_heads * a.head_dim * 2;
+        return a.clear_rest == 0 || cudaMemsetAsync(a.out, 0, bytes, static_cast<cudaStream_t>(stream)) == cudaSuccess ? EPTQ_OK : EPTQ_ERR_LAUNCH;
+    }
     const AttentionPlan plan = plan_of(a);
     if (plan.may_cut && (workspace == nullptr || workspace_bytes < bytes_of(a, plan))) return EPTQ_ERR_WORKSPACE;
     if (plan.may_cut && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return EPTQ_ERR_ALIGN;
@@ -194,6 +199,7 @@ extern "C" int eptq_ragged_attention(const EptqAttention* args, void* workspace,
     // A scale of zero stays a step above it: masked scores are -infinity and must stay so.
     p.scale_log2 = a.scale == 0.f ? 1e-30f : (a.scale < 0.f ? -a.scale : a.scale) * kLog2e;
     p.negative = a.scale < 0.f;
+    p.clear_rest = a.clear_rest != 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int status = on_tensor_cores(a) ? launch_attention_tcgen05(a, p, dev, st) : launch_attention_rows(a, p, dev, st);
     return status != EPTQ_OK || !plan.may_cut ? status : launch_join(a, plan, p, st);

@@ -423,7 +423,7 @@ int eptq_rope_append_paged(int dtype, const uint16_t* q, int64_t q_stride, const
  *   page_size == 0: k and v (rows, n_kv_heads*head_dim) are packed like q, and row t sees the rows 0 .. t of
  *     its request.
  * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads); sums, maxima and
- * products accumulate in 32 bits.  Rows behind the last request are left as they were.  head_dim 64 or 128.
+ * products accumulate in 32 bits.  Rows of no request are left as they were, or zeros with clear_rest.  head_dim 64 or 128.
  * Keys of a paged request are at most table_width * page_size: a larger kv_lens[b] counts as that.
  * Scratch: eptq_ragged_attention_workspace_bytes (0: none needed), 256-byte aligned, of any contents; calls that
  * may overlap on the GPU need scratch of their own.
@@ -435,7 +435,7 @@ typedef struct EptqAttention {
     int32_t max_rows;                  /* most rows of one request: chooses the kernel, not the result   */
     int32_t page_size, n_pages, table_width;          /* paged only                                     */
     float scale;
-    int32_t reserved;
+    int32_t clear_rest;                /* not 0: rows of no request become zeros instead of being left as they were */
     int64_t q_stride, k_stride, v_stride;             /* elements from row to row; paged: k, v page to page */
     int64_t table_stride;
     const uint16_t *q, *k, *v;
