@@ -41,6 +41,12 @@ int dtype_of(const at::Tensor& q, const char* what) {
 
 bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0; }
 const uint16_t* data(const at::Tensor& t) { return static_cast<const uint16_t*>(t.const_data_ptr()); }
+// For what a call writes: copy-on-write storage gets memory of its own, and autograd and whoever else watches the version
+// learns of the change.
+uint16_t* mutable_data(const at::Tensor& t) { return static_cast<uint16_t*>(t.mutable_data_ptr()); }
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 int narrow(int64_t v, const char* name) {
     REFUSE_UNLESS(v >= INT32_MIN && v <= INT32_MAX, name, " is out of range");
     return static_cast<int>(v);
@@ -149,9 +155,11 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out[5] = {part(all, at::kInt, 4 * rows, B + 1), part(all, at::kInt, 4 * rows + B + 1, B), part(all, at::kLong, 0, rows),
                          part(all, at::kLong, rows, rows), part(all, at::kInt, 4 * rows + 2 * B + 1, 1)};
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
-    done(eptq_plan_pages(cached.const_data_ptr<int32_t>(), fresh.const_data_ptr<int32_t>(), batch, const_cast<int32_t*>(tables.const_data_ptr<int32_t>()), stride, width,
+    int32_t* const table = tables.mutable_data_ptr<int32_t>();
+    done(eptq_plan_pages(cached.const_data_ptr<int32_t>(), fresh.const_data_ptr<int32_t>(), batch, table, stride, width,
                          free_pages.const_data_ptr<int32_t>(), cap, n_free.const_data_ptr<int32_t>(), page_size, n_rows, out[0].data_ptr<int32_t>(),
                          out[1].data_ptr<int32_t>(), out[2].data_ptr<int64_t>(), out[3].data_ptr<int64_t>(), out[4].data_ptr<int32_t>(), stream.stream()), "plan_pages");
+    written(tables);
     THPObjectPtr r(PyTuple_New(5));
     if (!r) return nullptr;
     for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(r.get(), i, THPVariable_Wrap(std::move(out[i])));
@@ -187,10 +195,13 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::OptionalCUDAGuard guard(device);
     at::Tensor out = output(a[9], q);
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
-    done(eptq_rope_append_paged(dtype, data(q), qs, data(k), ks, data(v), vs, static_cast<uint16_t*>(out.data_ptr()),
-                                const_cast<uint16_t*>(data(k_cache)), const_cast<uint16_t*>(data(v_cache)), c.stride, positions.const_data_ptr<int64_t>(),
+    uint16_t *const out_at = mutable_data(out), *const kc = mutable_data(k_cache), *const vc = mutable_data(v_cache);
+    done(eptq_rope_append_paged(dtype, data(q), qs, data(k), ks, data(v), vs, out_at, kc, vc, c.stride, positions.const_data_ptr<int64_t>(),
                                 slots.const_data_ptr<int64_t>(), inv_freq.const_data_ptr<float>(), narrow(rows, "the number of rows"), narrow(q.size(1) / c.head_dim, "the number of heads"),
                                 c.heads, c.head_dim, c.n_pages, c.page_size, scaling, stream.stream()), "rope_append_paged");
+    written(k_cache);
+    written(v_cache);
+    if (a[9] != Py_None) written(out);
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
@@ -204,9 +215,9 @@ PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const 
     a.batch = narrow(cu_rows.numel() - 1, "the number of requests");
     a.scale = static_cast<float>(scale == Py_None ? 1.0 / std::sqrt(static_cast<double>(a.head_dim)) : number(scale));
     a.q_stride = q_stride;
+    a.out = mutable_data(out);
     a.q = data(q);
     a.cu_rows = cu_rows.const_data_ptr<int32_t>();
-    a.out = static_cast<uint16_t*>(out.data_ptr());
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
     // Scratch of its own for every call, from torch's allocator: calls on different streams, and graphs captured on one
     // stream and replayed on others, share none.  The status word is that of the stream's scratch.
@@ -214,6 +225,7 @@ PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const 
     const size_t need = eptq_ragged_attention_workspace_bytes(&a);
     const at::Tensor ws = need == 0 ? at::Tensor() : at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
     done(eptq_ragged_attention(&a, need == 0 ? nullptr : ws.data_ptr(), need, stream.stream()), what);
+    if (out_or_none != Py_None) written(out);
     return THPVariable_Wrap(std::move(out));
 }
 

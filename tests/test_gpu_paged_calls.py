@@ -55,3 +55,75 @@ def test_rows_of_no_prompt_are_zeros_without_out():
     assert bool((paged.prompt_attention(q, k, v, cu[:1], 128) == 0).all())                    # no prompt at all
     kept = torch.full_like(q, 9.0)
     assert bool((paged.prompt_attention(q, k, v, cu[:1], 128, out=kept) == 9).all())
+
+
+# ---- what is written is marked as written --------------------------------------------------------------------------
+def _append_case(rows=4, nh=4, nkv=2, hd=64, ps=16):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    q, k, v = (torch.randn(rows, n * hd, generator=g, device="cuda").half() for n in (nh, nkv, nkv))
+    kc, vc = (torch.zeros(3, nkv, ps, hd, dtype=FP16, device="cuda") for _ in range(2))
+    pos = torch.arange(rows, device="cuda")
+    return q, k, v, kc, vc, pos, pos + ps, 1.0 / (10000.0 ** (torch.arange(0, hd, 2, device="cuda").float() / hd))
+
+
+def _plan_case():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")            # noqa: E731
+    return [i32([0, 3]), i32([20, 1]), i32([[-1, -1], [2, -1]]), i32([0, 1, 3]), i32([3]), 16, 21]
+
+
+def test_versions_of_written_tensors_move():
+    from eptq_b200.kernels import paged
+    q, k, v, kc, vc, pos, slots, inv = _append_case()
+    both = torch.zeros(2, *kc.shape, dtype=FP16, device="cuda")
+    before = q._version, kc._version, vc._version, both._version
+    assert paged.rope_append_paged(q, k, v, kc, vc, pos, slots, inv, out=q) is q
+    assert q._version > before[0] and kc._version > before[1] and vc._version > before[2]
+    paged.rope_append_paged(q, k, v, both[0], both[1], pos, slots, inv)
+    assert both._version > before[3]                                            # through views
+    plan = _plan_case()
+    versions = [t._version for t in plan[:5]]
+    paged.plan_pages(*plan)
+    assert [t._version > v for t, v in zip(plan[:5], versions)] == [False, False, True, False, False]
+    s = make_step([(20, 2)], 4, 2, 64, 16, FP16, seed=1)
+    out = torch.zeros_like(s["q"])
+    version = out._version, s["k_cache"]._version
+    _attend(s, out=out)
+    assert out._version > version[0] and s["k_cache"]._version == version[1]
+    version = out._version
+    paged.prompt_attention(s["q"], k[:2], v[:2], s["cu_rows"], 64, out=out)
+    assert out._version > version
+
+
+def test_autograd_sees_an_overwritten_tensor():
+    w = torch.ones(2, 256, dtype=FP16, device="cuda", requires_grad=True)
+    s = make_step([(20, 2)], 4, 2, 64, 16, FP16, seed=1)
+    out = torch.ones_like(s["q"])
+    y = (w * out).sum()
+    _attend(s, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_a_lazy_copy_keeps_its_values():
+    from eptq_b200.kernels import paged
+    q, k, v, kc, vc, pos, slots, inv = _append_case()
+    copies = [torch._lazy_clone(t) for t in (q, kc, vc)]
+    want = [t.clone() for t in (q, kc, vc)]
+    paged.rope_append_paged(q, k, v, kc, vc, pos, slots, inv, out=q)
+    assert all(torch.equal(c, w) for c, w in zip(copies, want))
+    assert not torch.equal(q, want[0]) and bool((kc[1, :, :4] != 0).any()) and torch.equal(vc[1, :, :4].transpose(0, 1).reshape(4, -1), v)
+    plan = _plan_case()
+    copy, old = torch._lazy_clone(plan[2]), plan[2].clone()
+    paged.plan_pages(*plan)
+    assert torch.equal(copy, old) and plan[2].tolist() == [[3, 1], [2, -1]]
+
+
+def test_tensors_made_in_inference_mode():
+    from eptq_b200.kernels import paged
+    with torch.inference_mode():
+        case, plan = _append_case(), _plan_case()
+        inside = paged.rope_append_paged(*case)
+        paged.plan_pages(*plan)
+    assert torch.equal(paged.rope_append_paged(*case), inside)
+    assert plan[2].tolist() == [[3, 1], [2, -1]]
+    paged.plan_pages(*plan)
