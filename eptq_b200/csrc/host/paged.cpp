@@ -4,6 +4,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "../../../include/eptq_b200.h"
@@ -20,12 +21,14 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
     return THPVariable_Unpack(o);
 }
 
-// On the GPU, on `device` where one is given, and without a gradient to form.
+// On the GPU, on `device` where one is given, and without a gradient to form, backward or forward.
 const at::Tensor& on_gpu(PyObject* o, const char* name, const c10::Device* device = nullptr) {
     const at::Tensor& t = tensor(o, name);
     REFUSE_UNLESS(t.is_cuda(), "`", name, "` must be a CUDA tensor (there is no CPU path)");
     REFUSE_UNLESS(device == nullptr || t.device() == *device, "`", name, "` is on ", t.device(), ", not on ", *device);
     REFUSE_UNLESS(!t.requires_grad() || !at::GradMode::is_enabled(), "`", name, "` wants a gradient, and the paged operators form none");
+    REFUSE_UNLESS(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), "`", name,
+                  "` carries a forward-mode tangent, and the paged operators form none");
     return t;
 }
 

@@ -127,3 +127,29 @@ def test_tensors_made_in_inference_mode():
     assert torch.equal(paged.rope_append_paged(*case), inside)
     assert plan[2].tolist() == [[3, 1], [2, -1]]
     paged.plan_pages(*plan)
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------
+def test_gradients_and_tangents_are_refused():
+    import torch.autograd.forward_ad as fwAD
+    from eptq_b200.kernels import paged
+    q, k, v, kc, vc, pos, slots, inv = _append_case()
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    want = paged.prompt_attention(q, k, v, cu, 64)
+    for i in range(3):
+        x = [q, k, v]
+        x[i] = x[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="gradient"):
+            paged.prompt_attention(*x, cu, 64)
+        with torch.no_grad():
+            assert torch.equal(paged.prompt_attention(*x, cu, 64), want)
+        with fwAD.dual_level():
+            x[i] = fwAD.make_dual([q, k, v][i], torch.ones_like([q, k, v][i]))
+            with pytest.raises(RuntimeError, match="tangent"):
+                paged.prompt_attention(*x, cu, 64)
+            with pytest.raises(RuntimeError, match="tangent"):
+                paged.rope_append_paged(*x, kc, vc, pos, slots, inv)
+            with torch.no_grad(), fwAD._set_fwd_grad_enabled(False):
+                assert torch.equal(paged.prompt_attention(*x, cu, 64), want)
+            assert torch.equal(paged.prompt_attention(q, k, v, cu, 64), want)
+    assert bool((kc == 0).all())
