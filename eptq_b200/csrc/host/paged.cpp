@@ -99,12 +99,31 @@ int64_t table_of(const at::Tensor& t, int64_t B) {
     return t.numel() != 0 && B > 1 ? t.stride(0) : t.size(1);
 }
 
-at::Tensor output(PyObject* o, const at::Tensor& q) {
+struct Input { const at::Tensor& t; const char* name; };
+
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    uintptr_t from[2], to[2];
+    const at::Tensor* const both[2] = {&a, &b};
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor& t = *both[i];
+        if (t.numel() == 0) return false;
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        from[i] = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        to[i] = from[i] + (last + 1) * t.element_size();
+    }
+    return from[0] < to[1] && from[1] < to[0];
+}
+
+// The output, in memory apart from what the call reads meanwhile; q itself will do, each of its rows is read before it is written.
+at::Tensor output(PyObject* o, const at::Tensor& q, std::initializer_list<Input> others) {
     if (o == Py_None) return at::empty(q.sizes(), q.options());
     const c10::Device device = q.device();
     const at::Tensor& out = on_gpu(o, "out", &device);
     REFUSE_UNLESS(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous() && aligned(out),
                   "`out` must be contiguous, of q's shape and type");
+    REFUSE_UNLESS((q.is_contiguous() && q.const_data_ptr() == out.const_data_ptr()) || !overlap(out, q), "`out` overlaps `q` and is not q itself");
+    for (const Input& i : others) REFUSE_UNLESS(!overlap(out, i.t), "`out` overlaps `", i.name, "`");
     return out;
 }
 
@@ -196,7 +215,8 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     whole(inv_freq, "inv_freq", at::kFloat, c.head_dim / 2);
     const float scaling = static_cast<float>(number(a[8]));
     const c10::cuda::OptionalCUDAGuard guard(device);
-    at::Tensor out = output(a[9], q);
+    REFUSE_UNLESS(rows == 0 || k_cache.numel() == 0 || k_cache.const_data_ptr() != v_cache.const_data_ptr(), "k_cache and v_cache are the same memory");
+    at::Tensor out = output(a[9], q, {{k, "k"}, {v, "v"}, {k_cache, "k_cache"}, {v_cache, "v_cache"}, {positions, "positions"}, {slots, "slots"}, {inv_freq, "inv_freq"}});
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
     uint16_t *const out_at = mutable_data(out), *const kc = mutable_data(k_cache), *const vc = mutable_data(v_cache);
     done(eptq_rope_append_paged(dtype, data(q), qs, data(k), ks, data(v), vs, out_at, kc, vc, c.stride, positions.const_data_ptr<int64_t>(),
@@ -209,10 +229,11 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const at::Tensor& cu_rows, PyObject* scale, PyObject* out_or_none, const char* what) {
+PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const at::Tensor& cu_rows, std::initializer_list<Input> others, PyObject* scale,
+                 PyObject* out_or_none, const char* what) {
     const c10::Device device = q.device();
     const c10::cuda::OptionalCUDAGuard guard(device);
-    at::Tensor out = output(out_or_none, q);
+    at::Tensor out = output(out_or_none, q, others);
     a.clear_rest = out_or_none == Py_None;          // memory of the allocator's: rows of no request would show what it held
     a.rows = narrow(q.size(0), "the number of rows");
     a.batch = narrow(cu_rows.numel() - 1, "the number of requests");
@@ -271,7 +292,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.v = data(v_cache);
     p.tables = tables.const_data_ptr<int32_t>();
     p.kv_lens = kv_lens.const_data_ptr<int32_t>();
-    return attend(p, q, q_stride, cu_rows, a[7], a[8], "paged_attention");
+    return attend(p, q, q_stride, cu_rows, {{k_cache, "k_cache"}, {v_cache, "v_cache"}, {tables, "tables"}, {kv_lens, "kv_lens"}, {cu_rows, "cu_rows"}}, a[7], a[8],
+                  "paged_attention");
     END_HANDLE_TH_ERRORS
 }
 
@@ -300,7 +322,7 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.max_rows = narrow(q.size(0), "the number of rows");
     p.k = data(k);
     p.v = data(v);
-    return attend(p, q, q_stride, cu_rows, a[5], a[6], "prompt_attention");
+    return attend(p, q, q_stride, cu_rows, {{k, "k"}, {v, "v"}, {cu_rows, "cu_rows"}}, a[5], a[6], "prompt_attention");
     END_HANDLE_TH_ERRORS
 }
 

@@ -53,7 +53,7 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
                       positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor, scaling: float = 1.0,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary embedding of packed q and k (rows, heads * head_dim) and the store of k and v at `slots` of the caches;
-    returns the rotated q (`out`, which may be q itself, or a new tensor).  Pairs (i, i + head_dim / 2), angle
+    returns the rotated q (`out`, which may be q itself but overlaps nothing else, or a new tensor).  Pairs (i, i + head_dim / 2), angle
     positions[r] * inv_freq[i] formed in 64 bits, cos and sin kept in 32.  q, k and v may be column ranges of one
     projection's output.  A slot outside the cache (-1: a row without one) is not written; slots differ otherwise, or
     the slot holds a mixture."""
@@ -67,8 +67,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of q (rows, n_heads * head_dim), they are the last of its kv_lens[b] keys, and row t of n sees the keys
     0 .. kv_lens[b] - n + t.  One row per request while tokens are generated, many for a chunk of a prompt, both in one
     call.  `max_rows`: the most rows that one request has; it chooses the kernel and changes no result but its rounding.
-    Rows that see no key come out as zeros, rows of no request as they were in `out`, which overlaps no cache, and as zeros
-    without one.  A page id outside the cache stands for keys that are not there; kv_lens[b] counts as what the table's
+    Rows that see no key come out as zeros, rows of no request as they were in `out` (q itself, or memory of its own), and
+    as zeros without one.  A page id outside the cache stands for keys that are not there; kv_lens[b] counts as what the table's
     width holds at most."""
     return _lib.host().paged_attention(q, k_cache, v_cache, tables, kv_lens, cu_rows, max_rows, scale, out)
 
@@ -77,6 +77,6 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_rows:
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention inside each of many prompts packed into one call: q (rows, n_heads * head_dim), k and v
     (rows, n_kv_heads * head_dim), prompt b in the rows cu_rows[b] .. cu_rows[b+1]-1.  q, k and v may be column ranges of
-    one projection's output.  Rows of no prompt stay as they were in `out`, which overlaps neither k nor v, and are zeros
-    without one."""
+    one projection's output.  Rows of no prompt stay as they were in `out` (q itself, or memory of its own), and are
+    zeros without one."""
     return _lib.host().prompt_attention(q, k, v, cu_rows, head_dim, scale, out)

@@ -153,3 +153,46 @@ def test_gradients_and_tangents_are_refused():
                 assert torch.equal(paged.prompt_attention(*x, cu, 64), want)
             assert torch.equal(paged.prompt_attention(q, k, v, cu, 64), want)
     assert bool((kc == 0).all())
+
+
+def test_outputs_that_overlap_are_refused():
+    from eptq_b200.kernels import paged
+    q, k, v, kc, vc, pos, slots, inv = _append_case(nh=2)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    flat = torch.zeros(5 * 128, dtype=FP16, device="cuda")
+    shifted, ahead = flat[128:].view(4, 128), flat[:-128].view(4, 128)
+    for out, what in ((k, "k"), (v, "v"), (kc.view(-1)[:512].view(4, 128), "k_cache"), (vc.view(-1)[-512:].view(4, 128), "v_cache")):
+        with pytest.raises(RuntimeError, match=f"`out` overlaps `{what}`"):
+            paged.rope_append_paged(q, k, v, kc, vc, pos, slots, inv, out=out)
+    with pytest.raises(RuntimeError, match="`out` overlaps `q`"):
+        paged.rope_append_paged(shifted, k, v, kc, vc, pos, slots, inv, out=ahead)
+    with pytest.raises(RuntimeError, match="the same memory"):
+        paged.rope_append_paged(q, k, v, kc, kc, pos, slots, inv)
+    for out, what in ((k, "k"), (v, "v")):
+        with pytest.raises(RuntimeError, match=f"`out` overlaps `{what}`"):
+            paged.prompt_attention(q, k, v, cu, 64, out=out)
+    with pytest.raises(RuntimeError, match="`out` overlaps `q`"):
+        paged.prompt_attention(shifted, k, v, cu, 64, out=ahead)
+    wide = torch.zeros(4, 512, dtype=FP16, device="cuda")
+    with pytest.raises(RuntimeError, match="`out` overlaps `q`"):
+        paged.prompt_attention(wide[:, :128], k, v, cu, 64, out=wide.view(-1)[:512].view(4, 128))
+    tables, kv = torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda")
+    for out, what in ((kc.view(-1)[:512].view(4, 128), "k_cache"), (vc.view(-1)[-512:].view(4, 128), "v_cache")):
+        with pytest.raises(RuntimeError, match=f"`out` overlaps `{what}`"):
+            paged.paged_attention(q, kc, vc, tables, kv, cu, 4, out=out)
+    torch.cuda.synchronize()
+    assert bool((kc == 0).all()) and bool((vc == 0).all())
+
+
+@pytest.mark.parametrize("told", [1, 100000])
+def test_attention_in_place_of_q(told):
+    """Tiles that are cut and tiles that are not."""
+    from eptq_b200.kernels import paged
+    s = make_step([(9000, 21), (40, 40), (333, 1)], 8, 2, 128, 16, FP16, seed=4)
+    want = _attend(s, max_rows=told)
+    assert _attend(s, max_rows=told, out=s["q"]) is s["q"] and torch.equal(s["q"], want)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(3000, n * 64, generator=g, device="cuda").half() for n in (4, 2, 2))
+    cu = torch.tensor([0, 700, 3000], dtype=torch.int32, device="cuda")
+    want = paged.prompt_attention(q, k, v, cu, 64)
+    assert paged.prompt_attention(q, k, v, cu, 64, out=q) is q and torch.equal(q, want)
