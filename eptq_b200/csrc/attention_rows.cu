@@ -186,6 +186,9 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int c = 0; c < 2; ++c)
                     q[k][2 * c + e] = live ? *reinterpret_cast<const unsigned*>(src + k * 16 + c * 8) : 0u;
         }
+        // Up to eight rows leave the tile's upper eight to the second parts of their weights (see below).
+        const bool folded = p.heads_per_tile * min(it.tokens, tile_tokens) <= 8;
+        if (folded) seen[1] = seen[0];
         float o[HD / 8][4], top[2], bias[2], sum[2];
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -237,12 +240,14 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 any |= top[e] == -INFINITY ? high[e] > -INFINITY : (high[e] - top[e]) * p.scale_log2 > kRescaleAt;
             }
             if (__any_sync(0xffffffffu, any)) {
+                float lower = 1.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const bool none = top[e] == -INFINITY;
                     const bool moves = none ? high[e] > -INFINITY : (high[e] - top[e]) * p.scale_log2 > kRescaleAt;
                     const float new_bias = moves ? high[e] * p.scale_log2 - kExpOffset : bias[e];
-                    const float keep = none ? 1.f : exp2_approx(bias[e] - new_bias);
+                    float keep = none ? 1.f : exp2_approx(bias[e] - new_bias);
+                    if (e == 0) lower = keep; else if (folded) keep = lower;
                     top[e] = moves ? high[e] : top[e];
                     bias[e] = new_bias;
                     sum[e] *= keep;
@@ -250,16 +255,32 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     for (int n = 0; n < HD / 8; ++n) { o[n][2 * e] *= keep; o[n][2 * e + 1] *= keep; }
                 }
             }
-            unsigned w[kSub][4];
+            // A weight meets its value as the sum of two 16-bit values, which keeps 22 bits of it (16 where they are bf16).  The second
+            // ones take a product of their own, or where the tile has no more than eight rows the upper rows of the first.
+            unsigned w[kSub][4], rest[kSub][4] = {};
+            if (folded) {
 #pragma unroll
-            for (int n = 0; n < 2 * kSub; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float a = exp2_approx(fmaf(z[n][2 * e], p.scale_log2, -bias[e]));
-                    const float b = exp2_approx(fmaf(z[n][2 * e + 1], p.scale_log2, -bias[e]));
-                    sum[e] += a + b;
-                    w[n >> 1][(n & 1) * 2 + e] = Pair16<T>::pack(a, b);
+                for (int n = 0; n < 2 * kSub; ++n) {
+                    const float a = exp2_approx(fmaf(z[n][0], p.scale_log2, -bias[0]));
+                    const float b = exp2_approx(fmaf(z[n][1], p.scale_log2, -bias[0]));
+                    sum[0] += a + b;
+                    const uint2 both = Pair16<T>::split(a, b);
+                    w[n >> 1][(n & 1) * 2] = both.x;
+                    w[n >> 1][(n & 1) * 2 + 1] = both.y;
                 }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 2 * kSub; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float a = exp2_approx(fmaf(z[n][2 * e], p.scale_log2, -bias[e]));
+                        const float b = exp2_approx(fmaf(z[n][2 * e + 1], p.scale_log2, -bias[e]));
+                        sum[e] += a + b;
+                        const uint2 both = Pair16<T>::split(a, b);
+                        w[n >> 1][(n & 1) * 2 + e] = both.x;
+                        rest[n >> 1][(n & 1) * 2 + e] = both.y;
+                    }
+            }
             // Values behind the last key a row sees may be anything, and a weight of zero must make them zero: what lies
             // behind the last token's is cleared.  Where the tokens see different keys of this unit and a value is not finite,
             // every token's rows take their own product.
@@ -281,11 +302,19 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const float2 end = Pair16<T>::unpack(acc);
                 apart = __any_sync(0xffffffffu, end.x != end.x || end.y != end.y);
             }
-            if (!apart) {
-                product<T, HD, false>(o, w, v_at, tail, it.keys - key0, true, true);
-            } else {
-                for (int token = 0; token < min(it.tokens, tile_tokens); ++token)
-                    product<T, HD, true>(o, w, v_at, true, it.seen + token + 1 - key0, seen[0] == it.seen + token, seen[1] == it.seen + token);
+#pragma unroll 1
+            for (int part = folded ? 1 : 0;; ++part) {              // a loop, not twice the code: short calls wait for their instructions
+                if (!apart) {
+                    product<T, HD, false>(o, w, v_at, tail, it.keys - key0, true, true);
+                } else {
+                    for (int token = 0; token < min(it.tokens, tile_tokens); ++token)
+                        product<T, HD, true>(o, w, v_at, true, it.seen + token + 1 - key0, seen[0] == it.seen + token, seen[1] == it.seen + token);
+                }
+                if (part == 1) break;
+#pragma unroll
+                for (int b = 0; b < kSub; ++b)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) w[b][c] = rest[b][c];
             }
             __syncwarp();                                       // all lanes have read the stage
             if (i + kStages < units) {
@@ -298,6 +327,10 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         // the four warps' results meet; each lies where its stages were
         if (ok) {
             float* const mine = reinterpret_cast<float*>(ring);
+            if (folded) {
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n) { o[n][0] += o[n][2]; o[n][1] += o[n][3]; }
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = e * 8 + g;

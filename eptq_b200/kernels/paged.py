@@ -67,6 +67,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of q (rows, n_heads * head_dim), they are the last of its kv_lens[b] keys, and row t of n sees the keys
     0 .. kv_lens[b] - n + t.  One row per request while tokens are generated, many for a chunk of a prompt, both in one
     call.  `max_rows`: the most rows that one request has; it chooses the kernel and changes no result but its rounding.
+    Scores, maxima and sums are held in 32 bits.  Weights meet the values as two 16-bit numbers in the kernel for few rows
+    (`max_rows` times the heads of a key/value head up to 16), rounded to the inputs' type in the one for many.
     Rows that see no key come out as zeros, rows of no request as they were in `out` (q itself, or memory of its own), and
     as zeros without one.  A page id outside the cache stands for keys that are not there; kv_lens[b] counts as what the table's
     width holds at most."""
@@ -78,5 +80,5 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_rows:
     """Causal attention inside each of many prompts packed into one call: q (rows, n_heads * head_dim), k and v
     (rows, n_kv_heads * head_dim), prompt b in the rows cu_rows[b] .. cu_rows[b+1]-1.  q, k and v may be column ranges of
     one projection's output.  Rows of no prompt stay as they were in `out` (q itself, or memory of its own), and are
-    zeros without one."""
+    zeros without one.  Weights are rounded to the inputs' type before they meet the values; all else is held in 32 bits."""
     return _lib.host().prompt_attention(q, k, v, cu_rows, head_dim, scale, out)

@@ -422,8 +422,10 @@ int eptq_rope_append_paged(int dtype, const uint16_t* q, int64_t q_stride, const
  *     outside the cache do not count.
  *   page_size == 0: k and v (rows, n_kv_heads*head_dim) are packed like q, and row t sees the rows 0 .. t of
  *     its request.
- * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads); sums, maxima and
- * products accumulate in 32 bits.  Rows of no request are left as they were, or zeros with clear_rest.  head_dim 64 or 128.
+ * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads).  Scores, maxima, sums and
+ * outputs accumulate in 32 bits; the weights meet the values rounded to the inputs' type, or as two 16-bit numbers
+ * (22 bits, 16 of bf16) where max_rows * n_heads / n_kv_heads of a paged call is at most 16.  Rows of no request are
+ * left as they were, or zeros with clear_rest.  head_dim 64 or 128.
  * Keys of a paged request are at most table_width * page_size: a larger kv_lens[b] counts as that.
  * Scratch: eptq_ragged_attention_workspace_bytes (0: none needed), 256-byte aligned, of any contents; calls that
  * may overlap on the GPU need scratch of their own.
