@@ -161,7 +161,7 @@ struct AppendArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_paged_kernel(const AppendArgs p) {
-    __shared__ float cos_s[kAppendMaxHeadDim / 2], sin_s[kAppendMaxHeadDim / 2];
+    __shared__ __align__(16) float cos_s[kAppendMaxHeadDim / 2], sin_s[kAppendMaxHeadDim / 2];      // read in pairs
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long r = blockIdx.x;
