@@ -30,7 +30,9 @@ namespace {
 // Block (share, 16 rows of its cut tile), 8 columns of one row per thread.  Where the tile has 8 rows or 4 -- a long request of one
 // token has 50 pieces of 4 rows -- two or four sets of threads take every second or fourth piece.  Pieces are added in an order
 // that depends on the tile and its cuts alone.  About 4 us where little is cut (launch, descriptor, reads in turn), 7 us for 55
-// pieces of 8 tiles of 4 rows, 13 us for a cut tile of 256 rows in every share (80 MB through L2).
+// pieces of 8 tiles of 4 rows, 13 us for a cut tile of 256 rows in every share (39 MB of pieces).  Where a tile has fewer pieces than are
+// read together, its last one is read for those it lacks: branches around the reads made calls of 24.2, 40.7 and 32.1 us (32 rows
+// on 6000 keys, 5 times 64 on 3000, 256 on 2000; 32 over 8 heads) 24.8, 44.1 and 35.3 us.
 constexpr int kJoinRows = 16;
 
 template <typename T, int HD>
