@@ -38,6 +38,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 constexpr size_t kCounterBytes = 4096;
 constexpr size_t kPartialOffset = 1u << 20;
 constexpr int kMaxCounters = static_cast<int>(kCounterBytes / sizeof(unsigned));
+static_assert(EPTQ_STATUS_BYTE == (kMaxCounters - 1) * sizeof(unsigned), "the status word is the last counter");
 constexpr int kGemmMinBatch = 16;           // batches above this run on the tensor-core GEMM
 // From kDenseMinTokens on the weight is reconstructed once into scratch and a dense GEMM follows, if the scratch has room
 // (eptq_layer_workspace_bytes asks for it).  Up to 512 tokens one token tile reads each weight once anyway, and there K

@@ -12,8 +12,6 @@
 
 namespace {
 
-constexpr size_t kStatusWord = 4092;      // byte of a scratch tensor's status word: the last of its counters
-
 #define REFUSE_UNLESS(cond, ...) TORCH_CHECK(cond, "eptq_b200: ", __VA_ARGS__)
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
@@ -245,7 +243,7 @@ PyObject* attend(EptqAttention& a, const at::Tensor& q, int64_t q_stride, const 
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
     // Scratch of its own for every call, from torch's allocator: calls on different streams, and graphs captured on one
     // stream and replayed on others, share none.  The status word is that of the stream's scratch.
-    a.status = reinterpret_cast<int32_t*>(static_cast<char*>(scratch_for(device.index(), stream, 1u << 20).data_ptr()) + kStatusWord);
+    a.status = reinterpret_cast<int32_t*>(static_cast<char*>(scratch_for(device.index(), stream, 1u << 20).data_ptr()) + EPTQ_STATUS_BYTE);
     const size_t need = eptq_ragged_attention_workspace_bytes(&a);
     const at::Tensor ws = need == 0 ? at::Tensor() : at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
     done(eptq_ragged_attention(&a, need == 0 ? nullptr : ws.data_ptr(), need, stream.stream()), what);

@@ -12,6 +12,10 @@ that get a chunk of their prompt:
 and `prompt_attention` where all keys are in the call itself.  Lengths and tables stay on the device: nothing here waits
 for the GPU, and a captured step can be replayed for other lengths.  As everywhere in this package there is no fallback
 (a CPU tensor raises), launches go to the current stream, and no gradient is formed (a tensor that wants one raises).
+
+Every wait inside the attention kernels is bounded (2 s).  One that runs out cannot raise, because no call waits for the GPU: it
+leaves a code in the status word of the stream's scratch, and the outputs are not valid.  `kernels.workspace_status_all(device)`
+reads and clears the words of all streams; a server asks for it where it waits for a step's tokens anyway.
 """
 from __future__ import annotations
 

@@ -294,12 +294,15 @@ int eptq_linear_forward_chain(const EptqLayer* layers, int n_layers, const EptqF
                               int B, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * The last counter word of a scratch buffer is its status word: a kernel whose
- * bounded device-side wait ran out (the chained and streaming GEMV, the prefill
- * GEMM) leaves EPTQ_ERR_TIMEOUT there and its output is not valid.  This copies
+ * The last counter word of a scratch buffer, EPTQ_STATUS_BYTE bytes behind its
+ * begin, is its status word: a kernel whose bounded device-side wait ran out (the
+ * chained and streaming GEMV, the prefill GEMM, and the ragged attention where its
+ * `status` points there, as from Python) leaves EPTQ_ERR_TIMEOUT there and its
+ * output is not valid.  This copies
  * the word to *host_out on `stream`, waits for that copy (it synchronises the
  * stream: do not call it during capture) and clears the word.
  */
+enum { EPTQ_STATUS_BYTE = 4092 };
 int eptq_workspace_status(void* workspace, int* host_out, void* stream);
 
 /*

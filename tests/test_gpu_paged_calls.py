@@ -196,3 +196,23 @@ def test_attention_in_place_of_q(told):
     cu = torch.tensor([0, 700, 3000], dtype=torch.int32, device="cuda")
     want = paged.prompt_attention(q, k, v, cu, 64)
     assert paged.prompt_attention(q, k, v, cu, 64, out=q) is q and torch.equal(q, want)
+
+
+# ---- waits that ran out ------------------------------------------------------------------------------------------------
+def test_status_word_of_the_stream_is_read():
+    """The word that the attention kernels are given is one that `workspace_status_all` reads: set here by hand, no wait runs out."""
+    from eptq_b200 import _lib
+    from eptq_b200.kernels import workspace_status_all
+    s = make_step([(20, 2), (300, 1)], 4, 2, 64, 16, FP16, seed=1)
+    device = s["q"].device
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for told in (1, 1000):
+            _attend(s, max_rows=told)
+        mine = _lib.host().scratch(device.index, 0)                                 # of this stream
+        assert mine.data_ptr() in {t.data_ptr() for t in _lib.host().scratch_of_device(device.index)}
+        assert workspace_status_all(device) == 0                                    # waits that did not run out
+        word = mine[4092:4096].view(torch.int32)
+        word.fill_(6)
+        assert workspace_status_all(device) == 6 and workspace_status_all(device) == 0 and int(word) == 0
