@@ -144,14 +144,19 @@ int check(const EptqAttention& a) {
     return EPTQ_OK;
 }
 
-// Up to 16 rows of one key/value head of a request fill the smallest matrix tile and the call is bound by the cache's reads;
-// above, the tcgen05 kernel reads as fast and multiplies faster: 32 rows over 4000 keys, 8 requests with 8 key/value heads,
-// 40 against 49 us (as two 16-row tiles), 64 rows over 1000 keys, 4 requests, 16 against 19 us; the other way round where heads
-// of 64 are many and short (20 rows over 1000 keys, 16 requests of 12 heads: 34 against 22 us).
-constexpr int kTensorRows = 16;
-
+// Tiles of 16 rows (whole tokens of one key/value head) up to which a request counts as few rows.  One is bound by the cache's reads; more
+// read the keys again, which pays as long as the smaller shares win more: with heads of 64 up to two tiles, with heads of 128 no longer.
+// Few rows against tcgen05, us, replayed:
+//   heads of 64, 32 rows: 12 heads, 16 requests of 1000 keys 30 / 40, 64 of 2000 138 / 161; 8 heads, 64 of 2000 98 / 122, 1 of 16000 25 / 24,
+//     16 of 1000 25 / 21; 40 rows: 39 / 40, 210 / 161, 136 / 122, 27 / 23, 28 / 21
+//   heads of 128, 16 rows: 12 heads, 16 of 1000 32 / 43, 64 of 2000 145 / 186; 8 heads, 64 of 2000 102 / 141, 1 of 16000 31 / 29, 16 of 1000
+//     26 / 26; 20 rows: 45 / 43, 268 / 189, 183 / 142, 36 / 29, 36 / 26
+// One or four short requests (1000 keys) would be faster with few rows at 64 rows still, 12 to 18 against 19 to 24 us, but lengths stand
+// on the device.
 bool on_tensor_cores(const EptqAttention& a) {
-    return a.page_size == 0 || static_cast<long long>(a.max_rows) * (a.n_heads / a.n_kv_heads) > kTensorRows;
+    const int group = a.n_heads / a.n_kv_heads, heads = heads_in(group, 16), tokens = 16 / heads;
+    const long long tiles = (static_cast<long long>(a.max_rows) + tokens - 1) / tokens * (group / heads);
+    return a.page_size == 0 || tiles > (a.head_dim == 64 ? 2 : 1);
 }
 
 AttentionPlan plan_of(const EptqAttention& a) { return on_tensor_cores(a) ? attention_tcgen05_plan(a) : attention_rows_plan(a); }

@@ -14,6 +14,16 @@ FP16, BF16 = torch.float16, torch.bfloat16
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (4, 4, 64), (16, 1, 64), (28, 4, 128)])
 @pytest.mark.parametrize("lens", [[(3, 1), (2, 1), (40, 1), (333, 1)] * 6, [(5, 2), (70, 2), (19, 1)] * 5])
 def test_weights_of_few_rows(dtype, nh, nkv, hd, lens):
+    _weights_of_few_rows(dtype, nh, nkv, hd, lens, 1)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,n", [(8, 2, 128, 4), (16, 1, 64, 2), (8, 8, 64, 32), (15, 5, 64, 10), (8, 8, 128, 16)])
+def test_most_rows_that_count_as_few(nh, nkv, hd, n):
+    """As many rows of a key/value head as the documentation names: a tile of 16, or two with heads of 64."""
+    _weights_of_few_rows(FP16, nh, nkv, hd, [(n + 3, n), (90, 1), (400, 2)] * 2, n)
+
+
+def _weights_of_few_rows(dtype, nh, nkv, hd, lens, max_rows):
     """The weight meets its value as two 16-bit values: the first cut off behind its last bit, so the second is below 2 steps of it and
     rounded by half a step of its own: 2 * 2^-11 * 2^-11 of the weight in fp16, 2 * 2^-8 * 2^-8 in bf16.  fp16 has a fixed step of
     2^-24 below its normal range: half a step of the first value and one of the second (which is not let become zero), of weights
@@ -22,7 +32,7 @@ def test_weights_of_few_rows(dtype, nh, nkv, hd, lens):
     from eptq_b200.kernels import paged
     s = make_step(lens, nh, nkv, hd, 16, dtype, seed=nh + hd + len(lens))
     s["q"] /= 16
-    got = paged.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["tables"], s["kv_lens"], s["cu_rows"], 1)
+    got = paged.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["tables"], s["kv_lens"], s["cu_rows"], max_rows)
     step, scale, at = HALF_STEP[dtype], hd ** -0.5, 0
     for b, (kv, n) in enumerate(lens):
         keys, values = (gather(s[c], s["tables"][b], kv).double() for c in ("k_cache", "v_cache"))
