@@ -11,6 +11,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstring>
@@ -117,6 +118,26 @@ std::vector<std::pair<int, at::Tensor>>& kept_scratch() {
     return *v;
 }
 
+bool is_capturing(cudaStream_t stream) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
+// Zeros that are there when it returns, also in a capture: that would record the zeroing for the graph's replays, each of which
+// would clear what other graphs and calls have left, and nothing would be zero before the first.  So it is done on a stream beside,
+// with memory of the ordinary pool.
+at::Tensor zeroed_scratch(int device, cudaStream_t stream, int64_t n) {
+    const auto options = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device));
+    if (!is_capturing(stream)) return at::zeros({n}, options);
+    c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, static_cast<c10::DeviceIndex>(device));
+    for (int i = 0; i < 64 && is_capturing(side.stream()); ++i) side = c10::cuda::getStreamFromPool(false, static_cast<c10::DeviceIndex>(device));
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    const c10::cuda::CUDAStreamGuard guard(side);
+    at::Tensor t = at::zeros({n}, options);
+    TORCH_CHECK(cudaStreamSynchronize(side.stream()) == cudaSuccess, "eptq_b200: the scratch of a captured stream could not be cleared");
+    return t;
+}
+
 }  // namespace
 
 at::Tensor scratch_for(int device, const c10::cuda::CUDAStream& stream, size_t bytes) {
@@ -127,13 +148,10 @@ at::Tensor scratch_for(int device, const c10::cuda::CUDAStream& stream, size_t b
             if (n < 2 * s.t.numel()) n = 2 * s.t.numel();
             kept_scratch().emplace_back(device, std::move(s.t));
         }
-        s.t = at::zeros({n}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+        s.t = zeroed_scratch(device, stream.stream(), n);
         s.captured = false;
     }
-    if (!s.captured) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        s.captured = cudaStreamIsCapturing(stream.stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
-    }
+    if (!s.captured) s.captured = is_capturing(stream.stream());
     return s.t;
 }
 

@@ -216,3 +216,29 @@ def test_status_word_of_the_stream_is_read():
         word = mine[4092:4096].view(torch.int32)
         word.fill_(6)
         assert workspace_status_all(device) == 6 and workspace_status_all(device) == 0 and int(word) == 0
+
+
+def test_scratch_made_in_a_capture():
+    """A stream's first call is a captured one: its scratch is zero at once, and no replay clears a code that stands there."""
+    from eptq_b200 import _lib
+    from eptq_b200.kernels import workspace_status_all
+    s = make_step([(20, 2), (300, 1)], 4, 2, 64, 16, FP16, seed=1)
+    want, device = _attend(s), s["q"].device
+    before = {t.data_ptr() for t in _lib.host().scratch_of_device(device.index)}
+    for _ in range(64):                                                             # a stream that has no scratch yet
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = _attend(s)
+        with torch.cuda.stream(stream):
+            mine = _lib.host().scratch(device.index, 0)
+        if mine.data_ptr() not in before:
+            break
+    else:
+        pytest.skip("every stream of the pool has scratch by now")
+    assert bool((mine[:1 << 20] == 0).all())                                        # before any replay
+    mine[4092:4096].view(torch.int32).fill_(6)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and workspace_status_all(device) == 6 and workspace_status_all(device) == 0
