@@ -8,9 +8,9 @@
 // shared memory.  Three blocks an SM cover each other's ends and starts (refilling on into the next tile, with shared memory
 // of its own for the results, was 5 to 8 % slower).  Which keys a block takes: attention_schedule.cuh.
 //
-// Measured on one B200, keys and values read by the call's time: 64 requests of 100 to 16000 keys, 32 over 8 heads of 128, 131 us
-// (5.8 TB/s); the same over 32 heads 476 us (6.4 TB/s); 256 requests of 100 to 1000 keys 76 us (5.4 TB/s); one request of 907
-// keys 9.9 us, which is launch, share, page table, first reads and the join.
+// Measured on one B200, replayed (join included), keys and values read by that time: 64 requests of 100 to 16000 keys, 32 over 8 heads
+// of 128, 132 us (5.8 TB/s); the same over 32 heads 477 us (6.4 TB/s); 256 requests of 100 to 1000 keys 76 us (5.4 TB/s); one request
+// of 907 keys 10.1 us, which is launch, share, page table, first reads and the join.
 
 #include <mutex>
 

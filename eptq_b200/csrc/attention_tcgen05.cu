@@ -19,8 +19,9 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8, by the softmax thread itself; P then stays below
 // 2^15 because exponents carry an offset of 7, which also keeps small weights out of fp16's subnormal range.
 //
-// Measured on one B200: prompt of 16384 tokens, 32 over 8 heads of 128, 1.77 ms (1240 TFLOP/s); 8191 tokens, 32 heads, 523 us
-// (1050 TFLOP/s); 509 rows of 64 over 8 heads on 24001 keys 392 us (1030 TFLOP/s); 1024 tokens 26 us.
+// Measured on one B200, calls back to back: prompt of 16384 tokens, 32 over 8 heads of 128, 1.73 ms (1270 TFLOP/s); 1024 tokens 26 us.
+// Replayed: 8191 tokens, 32 heads, bf16, 510 us (1080 TFLOP/s); 509 rows of 64 over 8 heads on 24001 keys 377 us (1070 TFLOP/s); over
+// seconds, under the power cap, 590 and 438 us.
 //
 // Keys behind a request's end are masked by index, whatever is stored there; their values would still meet a weight of
 // zero, so the product ends with the last key (in steps of 16, the rest of the last step cleared in shared memory).  Where a

@@ -18,7 +18,7 @@ namespace {
 // A few bytes per request and 16 per row: the time is the launch and the chain of dependent reads, so it is one launch.
 // Every block forms the sums over all requests itself, 1024 at a time (512 requests are 4 KB from L2), instead of
 // waiting for another block's, and then writes its share of the rows and pages, found by bisection in the sums.  4.6 us for 64
-// requests of one token, 6.1 us for 512 requests and 49904 rows, replayed.
+// requests of one token, 6.0 us for 512 requests and 49904 rows, replayed.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRowsPerBlock = 1024;
 
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanArgs
 // neighbouring pairs of one head (two 16-byte reads, two 16-byte writes).  The angle position * inv_freq is exact in 64
 // bits and reduced there to [-pi, pi]: in 32 bits it would be off by position * 2^-24, more than a rounding of the
 // outputs from a few thousand tokens on.  cos and sin stay in 32 bits: they are rounded once, with the product.  Bound by memory:
-// 4847 rows of 32 + 8 + 8 heads of 128 in 20.9 us (5.7 TB/s), 8 rows in 3.9 us.
+// 4847 rows of 32 + 8 + 8 heads of 128 in 21.0 us (5.7 TB/s), 8 rows in 3.9 us, replayed.  (Aligned
+// to 16 bytes, the pairs of cos and sin are read four at a time, and the same rows take 22.0 us.)
 constexpr int kAppendThreads = 128;
 constexpr int kAppendMaxHeadDim = 256;
 
@@ -161,7 +162,7 @@ struct AppendArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_paged_kernel(const AppendArgs p) {
-    __shared__ __align__(16) float cos_s[kAppendMaxHeadDim / 2], sin_s[kAppendMaxHeadDim / 2];      // read in pairs
+    __shared__ __align__(8) float cos_s[kAppendMaxHeadDim / 2], sin_s[kAppendMaxHeadDim / 2];      // read in pairs
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long r = blockIdx.x;
