@@ -29,7 +29,8 @@ __all__ = ["PagePlan", "plan_pages", "rope_append_paged", "paged_attention", "pr
 
 
 class PagePlan(NamedTuple):
-    """What `plan_pages` returns, all on the device: for B requests and `rows` rows of packed new tokens."""
+    """What `plan_pages` returns, all on the device: for B requests and `rows` rows of packed new tokens.  The five are parts of
+    one allocation, which lives as long as any of them."""
     cu_rows: torch.Tensor       # int32 (B + 1): rows cu_rows[b] .. cu_rows[b+1]-1 belong to request b
     kv_lens: torch.Tensor       # int32 (B): keys of the request with its new tokens, 0 where it was not served
     positions: torch.Tensor     # int64 (rows): a row's place in its request
