@@ -120,6 +120,7 @@ at::Tensor output(PyObject* o, const at::Tensor& q, std::initializer_list<Input>
     const at::Tensor& out = on_gpu(o, "out", &device);
     REFUSE_UNLESS(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous() && aligned(out),
                   "`out` must be contiguous, of q's shape and type");
+    out.mutable_data_ptr();                       // a lazy copy gets memory of its own here, apart from its original's
     REFUSE_UNLESS((q.is_contiguous() && q.const_data_ptr() == out.const_data_ptr()) || !overlap(out, q), "`out` overlaps `q` and is not q itself");
     for (const Input& i : others) REFUSE_UNLESS(!overlap(out, i.t), "`out` overlaps `", i.name, "`");
     return out;
@@ -213,10 +214,11 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     whole(inv_freq, "inv_freq", at::kFloat, c.head_dim / 2);
     const float scaling = static_cast<float>(number(a[8]));
     const c10::cuda::OptionalCUDAGuard guard(device);
-    REFUSE_UNLESS(rows == 0 || k_cache.numel() == 0 || k_cache.const_data_ptr() != v_cache.const_data_ptr(), "k_cache and v_cache are the same memory");
+    uint16_t *const kc = mutable_data(k_cache), *const vc = mutable_data(v_cache);
+    REFUSE_UNLESS(rows == 0 || k_cache.numel() == 0 || kc != vc, "k_cache and v_cache are the same memory");
     at::Tensor out = output(a[9], q, {{k, "k"}, {v, "v"}, {k_cache, "k_cache"}, {v_cache, "v_cache"}, {positions, "positions"}, {slots, "slots"}, {inv_freq, "inv_freq"}});
     const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
-    uint16_t *const out_at = mutable_data(out), *const kc = mutable_data(k_cache), *const vc = mutable_data(v_cache);
+    uint16_t* const out_at = mutable_data(out);
     done(eptq_rope_append_paged(dtype, data(q), qs, data(k), ks, data(v), vs, out_at, kc, vc, c.stride, positions.const_data_ptr<int64_t>(),
                                 slots.const_data_ptr<int64_t>(), inv_freq.const_data_ptr<float>(), narrow(rows, "the number of rows"), narrow(q.size(1) / c.head_dim, "the number of heads"),
                                 c.heads, c.head_dim, c.n_pages, c.page_size, scaling, stream.stream()), "rope_append_paged");

@@ -242,3 +242,15 @@ def test_scratch_made_in_a_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and workspace_status_all(device) == 6 and workspace_status_all(device) == 0
+
+
+def test_lazy_copies_of_inputs_are_outputs():
+    """A lazy copy shares its original's memory until it is written; that is no overlap."""
+    from eptq_b200.kernels import paged
+    q, k, v, kc, vc, pos, slots, inv = _append_case(nh=2)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    want = paged.prompt_attention(q, k, v, cu, 64)
+    old = k.clone()
+    assert torch.equal(paged.prompt_attention(q, k, v, cu, 64, out=torch._lazy_clone(k)), want) and torch.equal(k, old)
+    paged.rope_append_paged(q, k, v, kc, torch._lazy_clone(kc), pos, slots, inv)
+    assert bool((kc[1] != 0).any())
