@@ -59,9 +59,9 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary embedding of packed q and k (rows, heads * head_dim) and the store of k and v at `slots` of the caches;
     returns the rotated q (`out`, which may be q itself but overlaps nothing else, or a new tensor).  Pairs
-    (i, i + head_dim / 2), angle positions[r] * inv_freq[i] formed in 64 bits, cos and sin kept in 32.  q, k and v may be column ranges of one
-    projection's output.  A slot outside the cache (-1: a row without one) is not written; slots differ otherwise, or
-    the slot holds a mixture."""
+    (i, i + head_dim / 2), angle positions[r] * inv_freq[i] formed in 64 bits, cos and sin kept in 32.  q, k and v may be
+    column ranges of one projection's output.  A slot outside the cache (-1: a row without one) is not written; slots
+    differ otherwise, or the slot holds a mixture."""
     return _lib.host().rope_append_paged(q, k, v, k_cache, v_cache, positions, slots, inv_freq, scaling, out)
 
 
@@ -74,9 +74,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     call.  `max_rows`: the most rows that one request has; it chooses the kernel and changes no result but its rounding.
     Scores, maxima and sums are held in 32 bits.  Weights meet the values as two 16-bit numbers in the kernel for few rows
     (`max_rows` tokens of one key/value head in 16 rows, or twice that with heads of 64), rounded to the inputs' type in
-    the one for many.  Rows that see no key come out as zeros, rows of no request as they were in `out` (q itself, or memory of its own), and
-    as zeros without one.  A page id outside the cache stands for keys that are not there; kv_lens[b] counts as what the
-    table's width holds at most."""
+    the one for many.  Rows that see no key come out as zeros, rows of no request as they were in `out` (q itself, or
+    memory of its own), and as zeros without one.  A page id outside the cache stands for keys that are not there;
+    kv_lens[b] counts as what the table's width holds at most."""
     return _lib.host().paged_attention(q, k_cache, v_cache, tables, kv_lens, cu_rows, max_rows, scale, out)
 
 

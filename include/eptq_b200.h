@@ -428,7 +428,8 @@ int eptq_rope_append_paged(int dtype, const uint16_t* q, int64_t q_stride, const
  * out = softmax(scale * q k^T) v, head h with the keys of head h / (n_heads / n_kv_heads).  Scores, maxima, sums and
  * outputs accumulate in 32 bits; the weights meet the values rounded to the inputs' type, or as two 16-bit numbers
  * (22 bits, 16 of bf16) where max_rows tokens of one key/value head of a paged call fit a tile of 16 rows (two
- * tiles with heads of 64; a token's heads stay together).  Rows of no request are left as they were, or zeros with clear_rest.  head_dim 64 or 128.
+ * tiles with heads of 64; a token's heads stay together).  Rows of no request are left as they were, or zeros
+ * with clear_rest.  head_dim 64 or 128.
  * Keys of a paged request are at most table_width * page_size: a larger kv_lens[b] counts as that.
  * Scratch: eptq_ragged_attention_workspace_bytes (0: none needed), 256-byte aligned, of any contents; calls that
  * may overlap on the GPU need scratch of their own.
